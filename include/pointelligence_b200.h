@@ -451,6 +451,74 @@ int pcx_ragged_group_norm_backward(const void *d_grad_y, const void *d_x,
                                    int G, int dtype, void *d_ws, size_t ws_bytes,
                                    void *stream);
 
+/* Group normalisation over a ragged batch with what follows it in a residual
+ * block, in the same passes over the rows:
+ *   y = drop(act((x - mean_{s,g}) * rstd_{s,g} * weight + bias (+ residual)))
+ * G = 1 is the ragged layer norm, G = C the instance norm; C <= 65536.
+ * `activation`: a pcx_activation.  `dropout` is the probability of the dropout
+ * by element described at pcx_dropout (0: none).  d_weight / d_bias (fp32, C) may both
+ * be null, and so may d_residual.  d_mean / d_rstd (fp32, S * G, index s * G + g)
+ * are outputs kept for the backward pass, which makes the activation's argument and the
+ * mask again: give it the tensors, the probability and the seed of the forward
+ * call.  d_grad_weight / d_grad_bias (fp32, C) may both be null, and so may
+ * d_grad_residual.  Results do not depend on scheduling: sums are merged in a
+ * fixed order.  Lengths are taken within the rows there are; rows behind the
+ * last sample are its own.  (layers/norm.py:86-130 of the reference composes the
+ * norm; it has neither the activation nor the dropout in it.) */
+typedef enum {
+    PCX_ACT_NONE = 0,
+    PCX_ACT_RELU = 1,
+    PCX_ACT_SILU = 2, /* z / (1 + exp(-z)) */
+    PCX_ACT_GELU = 3  /* z (1 + erf(z / sqrt 2)) / 2 */
+} pcx_activation;
+size_t pcx_ragged_group_norm_act_workspace_bytes(int64_t N, int64_t S, int C,
+                                                 int G, int dtype);
+int pcx_ragged_group_norm_act(const void *d_x, const int64_t *d_lengths,
+                              const float *d_weight, const float *d_bias,
+                              const void *d_residual, void *d_y, float *d_mean,
+                              float *d_rstd, int64_t N, int64_t S, int C, int G,
+                              double eps, int activation, double dropout,
+                              uint64_t seed, uint64_t offset, const int64_t *d_rng,
+                              int dtype, void *d_ws, size_t ws_bytes, void *stream);
+int pcx_ragged_group_norm_act_backward(
+    const void *d_grad_y, const void *d_x, const void *d_residual,
+    const int64_t *d_lengths, const float *d_weight, const float *d_bias,
+    const float *d_mean, const float *d_rstd, void *d_grad_x, float *d_grad_weight,
+    float *d_grad_bias, void *d_grad_residual, int64_t N, int64_t S, int C, int G,
+    int activation, double dropout, uint64_t seed, uint64_t offset,
+    const int64_t *d_rng, int dtype, void *d_ws, size_t ws_bytes, void *stream);
+
+/* ------------------------------------------------------------------------
+ * Dropout with the tail of a residual block, its mask never stored:
+ *   y = relu?((residual +) keep[u] * x / (1 - p))
+ * `unit` (a pcx_drop_unit): what is dropped together.  Unit u is kept where
+ * word u % 8 (16 bits, low halves first) of Philox4x32-10 with the counter
+ * (u / 8, offset) and the key `seed` is at least t = round(65536 p), and scaled by
+ * 65536 / (65536 - t); what is dropped is zero whatever it was.  Elements are
+ * numbered row by row, channels of samples s * C + c.  d_rng, if not null,
+ * is two int64 on the device (seed, offset) that the kernel reads when it runs, instead
+ * of the two arguments: a captured graph can be replayed with others.
+ * d_lengths is read for channels and samples only (S samples), and so is the
+ * workspace; d_residual may be null.
+ * _backward: d_y, the forward result, is read only when relu != 0;
+ * d_grad_residual may be null.  No counterpart in the reference. */
+typedef enum { PCX_DROP_ELEMENT = 0, PCX_DROP_CHANNEL = 1, PCX_DROP_SAMPLE = 2 } pcx_drop_unit;
+size_t pcx_dropout_workspace_bytes(int64_t S, int unit);
+int pcx_dropout(const void *d_x, const int64_t *d_lengths, const void *d_residual,
+                void *d_y, int64_t N, int64_t S, int C, int unit, int relu,
+                double dropout, uint64_t seed, uint64_t offset, const int64_t *d_rng,
+                int dtype, void *d_ws, size_t ws_bytes, void *stream);
+int pcx_dropout_backward(const void *d_grad_y, const void *d_y,
+                         const int64_t *d_lengths, void *d_grad_x,
+                         void *d_grad_residual, int64_t N, int64_t S, int C, int unit,
+                         int relu, double dropout, uint64_t seed, uint64_t offset,
+                         const int64_t *d_rng, int dtype, void *d_ws, size_t ws_bytes,
+                         void *stream);
+/* d_rng = (*d_seed, *d_offset + more): the state of a generator that a graph is
+ * captured with, as the calls above read it. */
+int pcx_rng_state(const int64_t *d_seed, const int64_t *d_offset, int64_t more,
+                  int64_t *d_rng, void *stream);
+
 /* ------------------------------------------------------------------------
  * Tap bookkeeping.
  * pcx_seg_offs: seg[k] = first position with value >= k in a sorted int32

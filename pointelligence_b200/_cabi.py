@@ -13,7 +13,7 @@ import ctypes
 import os
 import threading
 import time
-from ctypes import c_double, c_int, c_int64, c_size_t, c_void_p
+from ctypes import c_double, c_int, c_int64, c_size_t, c_uint64, c_void_p
 
 import torch
 
@@ -93,6 +93,17 @@ SIGNATURES = {
                                                       c_size_t, c_void_p]),
     "pcx_ragged_layer_norm_backward": (c_int, [c_void_p] * 11 + [c_int64, c_int64, c_int, c_int, c_int, c_void_p,
                                                                 c_size_t, c_void_p]),
+    "pcx_ragged_group_norm_act_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int, c_int, c_int]),
+    "pcx_ragged_group_norm_act": (c_int, [c_void_p] * 8 + [c_int64, c_int64, c_int, c_int, c_double, c_int, c_double, c_uint64,
+                                  c_uint64, c_void_p, c_int, c_void_p, c_size_t, c_void_p]),
+    "pcx_ragged_group_norm_act_backward": (c_int, [c_void_p] * 12 + [c_int64, c_int64, c_int, c_int, c_int, c_double, c_uint64,
+                                           c_uint64, c_void_p, c_int, c_void_p, c_size_t, c_void_p]),
+    "pcx_dropout_workspace_bytes": (c_size_t, [c_int64, c_int]),
+    "pcx_dropout": (c_int, [c_void_p] * 4 + [c_int64, c_int64, c_int, c_int, c_int, c_double, c_uint64, c_uint64, c_void_p, c_int,
+                            c_void_p, c_size_t, c_void_p]),
+    "pcx_dropout_backward": (c_int, [c_void_p] * 5 + [c_int64, c_int64, c_int, c_int, c_int, c_double, c_uint64, c_uint64,
+                                     c_void_p, c_int, c_void_p, c_size_t, c_void_p]),
+    "pcx_rng_state": (c_int, [c_void_p] * 2 + [c_int64, c_void_p, c_void_p]),
     "pcx_ragged_group_norm_workspace_bytes": (c_size_t, [c_int64, c_int]),
     "pcx_ragged_group_norm": (c_int, [c_void_p] * 7 + [c_int64, c_int64, c_int, c_int, c_double, c_int, c_void_p,
                                                       c_size_t, c_void_p]),

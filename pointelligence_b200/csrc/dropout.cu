@@ -1,0 +1,251 @@
+// Dropout over a ragged batch with the tail of a residual block, its mask made by counting (philox.cuh) and never stored:
+//
+//   y = relu?((residual +) keep[u] * x / (1 - p))
+//
+// A unit u is an element (row-major index), a channel of a sample (s * C + c: feature dropout) or a sample (s: drop path, which
+// drops a residual branch whole).  Backward, with g masked where y > 0 does not hold (relu): dresidual = g, dx = keep[u] * g / (1 - p).
+// What is dropped is zero whatever it was, and rows of a dropped sample are not read.  Bound by bytes; by element a generator
+// call makes the words of eight elements, 7.5 operations each, beside the memory's work.
+#include <algorithm>
+
+#include "philox.cuh"
+#include "rowwise.cuh"
+
+namespace pcx {
+namespace {
+
+constexpr int DO_THREADS = 256;
+constexpr int DO_UNROLL = 4;                  // lumps a thread has in flight
+constexpr int DO_CHUNK_BYTES = 16 << 10;      // of rows, a block of the units' kernel
+
+struct DropArgs {
+    const void *x, *residual, *y_in;          // (backward: the gradient, none, the result for the ReLU)
+    void *y, *masked;                         // (backward: the input's gradient, the residual's)
+    const int64_t *offsets;
+    int64_t N, S;
+    int C, rows, relu;
+    Dropping drop;
+};
+
+template <typename T, int VN, bool BACKWARD>
+__device__ __forceinline__ void drop_lump(const DropArgs &p, int64_t at, const Lump<T, VN> &x, const Lump<T, VN> &other, const float *factor) {
+    Lump<T, VN> out;
+    if constexpr (BACKWARD) {
+        Lump<T, VN> g;
+#pragma unroll
+        for (int i = 0; i < VN; ++i) {
+            const float v = p.relu && !(other.get(i) > 0.f) ? 0.f : x.get(i);
+            g.set(i, v);
+            out.set(i, factor[i] > 0.f ? v * factor[i] : 0.f);
+        }
+        if (p.masked) g.store(static_cast<T *>(p.masked) + at);
+    } else {
+#pragma unroll
+        for (int i = 0; i < VN; ++i) {
+            float v = factor[i] > 0.f ? x.get(i) * factor[i] : 0.f;
+            if (p.residual) v += other.get(i);
+            out.set(i, p.relu ? relu(v) : v);
+        }
+    }
+    out.store(static_cast<T *>(p.y) + at);
+}
+
+// By element: a thread takes groups of eight consecutive ones, with the words of one call.
+// VN = 8: accesses of 16 bytes; 1: of one element, for tensors at other addresses.
+template <typename T, int VN, bool BACKWARD>
+__global__ void __launch_bounds__(DO_THREADS) drop_elements_kernel(const __grid_constant__ DropArgs p, int64_t n) {
+    start_after_previous();
+    const Philox rng(p.drop);
+    const T *x = static_cast<const T *>(p.x), *other = static_cast<const T *>(BACKWARD ? p.y_in : p.residual);
+    const bool reads = BACKWARD ? p.relu != 0 : p.residual != nullptr;
+    const int64_t g0 = (int64_t)blockIdx.x * (DO_THREADS * DO_UNROLL) + threadIdx.x;
+    if constexpr (VN == 8) {
+        Lump<T, 8> v[DO_UNROLL], q[DO_UNROLL];
+#pragma unroll
+        for (int u = 0; u < DO_UNROLL; ++u) {
+            const int64_t at = (g0 + u * DO_THREADS) * 8;
+            if (at + 8 <= n) {
+                v[u].load(x + at);
+                if (reads) q[u].load(other + at);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < DO_UNROLL; ++u) {
+            const int64_t at = (g0 + u * DO_THREADS) * 8;
+            if (at + 8 > n) break;
+            const uint32_t kept = p.drop.on ? rng.kept<8>((uint64_t)at, p.drop.over) : 0xff;
+            float f[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) f[i] = kept >> i & 1 ? p.drop.scale : 0.f;
+            drop_lump<T, 8, BACKWARD>(p, at, v[u], q[u], f);
+        }
+    }
+    for (int u = 0; u < DO_UNROLL; ++u) {   // one by one: all of them, or the last group's
+        const int64_t from = (g0 + u * DO_THREADS) * 8;
+        if (from >= n) break;
+        if (VN == 8 && from + 8 <= n) continue;
+        const uint32_t kept = p.drop.on ? rng.kept<8>((uint64_t)from, p.drop.over) : 0xff;
+        const int count = (int)min(n - from, (int64_t)8);
+        for (int i = 0; i < count; ++i) {
+            Lump<T, 1> v, q;
+            v.load(x + from + i);
+            if (reads) q.load(other + from + i);
+            const float f = kept >> i & 1 ? p.drop.scale : 0.f;
+            drop_lump<T, 1, BACKWARD>(p, from + i, v, q, &f);
+        }
+    }
+}
+
+// By channels of a sample, or by samples: a block has `rows` consecutive rows, and goes through them sample by sample.
+template <typename T, int VN, bool BACKWARD, bool SAMPLES>
+__global__ void __launch_bounds__(DO_THREADS) drop_units_kernel(const __grid_constant__ DropArgs p) {
+    start_after_previous();
+    const Philox rng(p.drop);
+    const T *x = static_cast<const T *>(p.x), *other = static_cast<const T *>(BACKWARD ? p.y_in : p.residual);
+    const bool reads = BACKWARD ? p.relu != 0 : p.residual != nullptr;
+    const int lumps = p.C / VN, cols = min(lumps, DO_THREADS), lanes = DO_THREADS / cols, col = threadIdx.x % cols, lane = threadIdx.x / cols;
+    const int64_t row0 = (int64_t)blockIdx.x * p.rows, row1 = min(p.N, row0 + p.rows);
+    if (lane >= lanes) return;
+    for (int64_t s = segment_of_row(p.offsets, p.S, row0); s < p.S && p.offsets[s] < row1; ++s) {
+        const int64_t lo = max(row0, p.offsets[s]), hi = min(row1, p.offsets[s + 1]);
+        if (hi <= lo) continue;
+        uint32_t kept = 0xff;
+        if (SAMPLES && p.drop.on) kept = rng.kept<1>((uint64_t)s, p.drop.over) ? 0xff : 0;
+        for (int lump = col; lump < lumps; lump += cols) {
+            const int c0 = lump * VN;
+            if (!SAMPLES && p.drop.on) kept = rng.kept<VN>((uint64_t)s * p.C + c0, p.drop.over);
+            const bool want = kept || (BACKWARD && p.masked);
+            float f[VN];
+#pragma unroll
+            for (int i = 0; i < VN; ++i) f[i] = kept >> i & 1 ? p.drop.scale : 0.f;
+            for (int64_t r = lo + lane; r < hi; r += (int64_t)DO_UNROLL * lanes) {
+                Lump<T, VN> v[DO_UNROLL], q[DO_UNROLL];
+#pragma unroll
+                for (int u = 0; u < DO_UNROLL; ++u) {
+                    const int64_t row = r + (int64_t)u * lanes, at = row * p.C + c0;
+#pragma unroll
+                    for (int w = 0; w < Lump<T, VN>::WORDS; ++w) v[u].w[w] = 0;
+                    if (row < hi) {
+                        if (want) v[u].load(x + at);
+                        if (reads) q[u].load(other + at);
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < DO_UNROLL; ++u) {
+                    const int64_t row = r + (int64_t)u * lanes;
+                    if (row < hi) drop_lump<T, VN, BACKWARD>(p, row * p.C + c0, v[u], q[u], f);
+                }
+            }
+        }
+    }
+}
+
+enum { UNIT_ELEMENT = 0, UNIT_CHANNEL = 1, UNIT_SAMPLE = 2 };
+
+template <typename T, bool BACKWARD>
+int run_elements(const DropArgs &p, bool wide, int64_t n, cudaStream_t stream) {
+    const unsigned grid = (unsigned)((n + 8 * DO_THREADS * DO_UNROLL - 1) / (8 * DO_THREADS * DO_UNROLL));
+    if (wide) launch_after(drop_elements_kernel<T, 8, BACKWARD>, grid, DO_THREADS, 0, stream, p, n);
+    else launch_after(drop_elements_kernel<T, 1, BACKWARD>, grid, DO_THREADS, 0, stream, p, n);
+    PCX_LAUNCH_CHECK();
+    return PCX_OK;
+}
+
+template <typename T, int VN, bool BACKWARD>
+int run_units(const DropArgs &p, int unit, cudaStream_t stream) {
+    const unsigned grid = (unsigned)((p.N + p.rows - 1) / p.rows);
+    if (unit == UNIT_SAMPLE) launch_after(drop_units_kernel<T, VN, BACKWARD, true>, grid, DO_THREADS, 0, stream, p);
+    else launch_after(drop_units_kernel<T, VN, BACKWARD, false>, grid, DO_THREADS, 0, stream, p);
+    PCX_LAUNCH_CHECK();
+    return PCX_OK;
+}
+
+template <typename T, bool BACKWARD>
+int run(const DropArgs &p, int unit, int vn, cudaStream_t stream) {
+    if (unit == UNIT_ELEMENT) return run_elements<T, BACKWARD>(p, vn == 8, p.N * p.C, stream);
+    if (vn == 8) return run_units<T, 8, BACKWARD>(p, unit, stream);
+    if (vn == 4) return run_units<T, 4, BACKWARD>(p, unit, stream);
+    if (vn == 2) return run_units<T, 2, BACKWARD>(p, unit, stream);
+    return run_units<T, 1, BACKWARD>(p, unit, stream);
+}
+
+size_t carve(void *ws, int64_t S, int unit, int64_t **offsets) {
+    Carver c(ws);
+    int64_t *at = c.take<int64_t>(unit == UNIT_ELEMENT ? 0 : (size_t)S + 1);
+    if (offsets) *offsets = at;
+    return c.off;
+}
+
+bool sizes_ok(int64_t N, int64_t S, int C, int unit, int dtype) {
+    return N >= 0 && C > 0 && unit >= UNIT_ELEMENT && unit <= UNIT_SAMPLE && (unit == UNIT_ELEMENT || (S > 0 && S <= INT32_MAX)) &&
+           (dtype == PCX_F32 || dtype == PCX_F16 || dtype == PCX_BF16) && N <= INT64_MAX / 8 / C && N * C / (8 * DO_THREADS) < INT32_MAX;
+}
+
+template <bool BACKWARD>
+int drop(const char *name, DropArgs p, const int64_t *d_lengths, int unit, double dropout, uint64_t seed, uint64_t offset, const int64_t *d_rng,
+         int dtype, void *d_ws, size_t ws_bytes, cudaStream_t stream) {
+    if (!sizes_ok(p.N, p.S, p.C, unit, dtype)) PCX_FAIL(PCX_E_ARG, "%s: bad sizes, unit or dtype", name);
+    if ((p.N > 0 && (!p.x || !p.y)) || (unit != UNIT_ELEMENT && (!d_lengths || !d_ws)) || (BACKWARD && p.relu && p.N > 0 && !p.y_in))
+        PCX_FAIL(PCX_E_ARG, "%s: null pointer", name);
+    if (!make_dropping(dropout, seed, offset, d_rng, &p.drop)) PCX_FAIL(PCX_E_ARG, "%s: %g is no probability", name, dropout);
+    if (p.N == 0) return PCX_OK;
+    const int vn = lump_of(unit == UNIT_ELEMENT ? 8 : p.C, dtype, {p.x, p.residual, p.y_in, p.y, p.masked});
+    prof_begin(BACKWARD ? "dropout(bwd)" : "dropout(fwd)", stream);
+    if (unit != UNIT_ELEMENT) {
+        if ((uintptr_t)d_ws % 256) PCX_FAIL(PCX_E_ALIGN, "%s: workspace must be 256-byte aligned", name);
+        int64_t *offsets = nullptr;
+        const size_t need = carve(d_ws, p.S, unit, &offsets);
+        if (ws_bytes < need) PCX_FAIL(PCX_E_CAPACITY, "%s: workspace %zu < %zu bytes", name, ws_bytes, need);
+        p.offsets = offsets;
+        const int64_t by_bytes = DO_CHUNK_BYTES / ((int64_t)p.C * (int64_t)elem_size(dtype)), by_chip = (p.N + 4 * num_sms() - 1) / (4 * num_sms());
+        p.rows = (int)std::max<int64_t>(1, std::min(by_bytes, by_chip));
+        if (p.N / p.rows >= INT32_MAX) PCX_FAIL(PCX_E_ARG, "%s: bad sizes, unit or dtype", name);
+        if (int rc = sample_offsets(d_lengths, offsets, p.S, p.N, stream)) return rc;
+    }
+    int rc = PCX_OK;
+    if (dtype == PCX_F32) rc = run<float, BACKWARD>(p, unit, vn, stream);
+    else if (dtype == PCX_F16) rc = run<__half, BACKWARD>(p, unit, vn, stream);
+    else rc = run<__nv_bfloat16, BACKWARD>(p, unit, vn, stream);
+    prof_end(stream);
+    return rc;
+}
+
+__global__ void rng_state_kernel(const int64_t *seed, const int64_t *offset, int64_t more, int64_t *out) {
+    start_after_previous();
+    if (threadIdx.x == 0) out[0] = *seed, out[1] = *offset + more;
+}
+
+}  // namespace
+}  // namespace pcx
+
+using namespace pcx;
+
+extern "C" {
+
+size_t pcx_dropout_workspace_bytes(int64_t S, int unit) {
+    return unit == UNIT_ELEMENT || S <= 0 || S > INT32_MAX ? 0 : carve(nullptr, S, unit, nullptr);
+}
+
+int pcx_dropout(const void *d_x, const int64_t *d_lengths, const void *d_residual, void *d_y, int64_t N, int64_t S, int C, int unit, int relu,
+                double dropout, uint64_t seed, uint64_t offset, const int64_t *d_rng, int dtype, void *d_ws, size_t ws_bytes, void *stream) {
+    DropArgs p = {};
+    p.x = d_x, p.residual = d_residual, p.y = d_y, p.N = N, p.S = S, p.C = C, p.relu = relu;
+    return drop<false>("pcx_dropout", p, d_lengths, unit, dropout, seed, offset, d_rng, dtype, d_ws, ws_bytes, (cudaStream_t)stream);
+}
+
+int pcx_dropout_backward(const void *d_grad_y, const void *d_y, const int64_t *d_lengths, void *d_grad_x, void *d_grad_residual, int64_t N, int64_t S,
+                         int C, int unit, int relu, double dropout, uint64_t seed, uint64_t offset, const int64_t *d_rng, int dtype, void *d_ws,
+                         size_t ws_bytes, void *stream) {
+    DropArgs p = {};
+    p.x = d_grad_y, p.y_in = relu ? d_y : nullptr, p.y = d_grad_x, p.masked = d_grad_residual, p.N = N, p.S = S, p.C = C, p.relu = relu;
+    return drop<true>("pcx_dropout_backward", p, d_lengths, unit, dropout, seed, offset, d_rng, dtype, d_ws, ws_bytes, (cudaStream_t)stream);
+}
+
+int pcx_rng_state(const int64_t *d_seed, const int64_t *d_offset, int64_t more, int64_t *d_rng, void *stream) {
+    if (!d_seed || !d_offset || !d_rng) PCX_FAIL(PCX_E_ARG, "pcx_rng_state: null pointer");
+    launch_after(rng_state_kernel, 1, 32, 0, (cudaStream_t)stream, d_seed, d_offset, more, d_rng);
+    PCX_LAUNCH_CHECK();
+    return PCX_OK;
+}
+
+}  // extern "C"

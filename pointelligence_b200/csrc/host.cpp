@@ -1,5 +1,5 @@
 // Host path of the hot operators: argument checks, output and workspace allocation, the C-ABI
-// calls and the autograd nodes of the convolution and the ragged layer norm, compiled.
+// calls and the autograd nodes of the convolution, the ragged norms and dropout, compiled.
 //
 // The kernels live behind the C ABI (include/pointelligence_b200.h).  What this file replaces is the
 // interpreter between a layer's forward() and those entry points: a training pass of one layer
@@ -13,6 +13,7 @@
 
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/CUDAEvent.h>
+#include <ATen/cuda/CUDAGeneratorImpl.h>
 #include <c10/cuda/CUDAGuard.h>
 
 #include "../../include/pointelligence_b200.h"
@@ -570,6 +571,264 @@ Tensor layer_norm(const Tensor &x, const Tensor &lengths, const OptTensor &weigh
     return LayerNorm::apply(x, lengths, weight, bias, residual, eps, relu);
 }
 
+// ------------------------------------------------ seeds of what is dropped at random ----
+// (seed, offset) of a dropout: two numbers, or an int64 tensor of them that the kernels read when they run.
+struct Rng {
+    uint64_t seed = 0, offset = 0;
+    OptTensor state;
+};
+
+// A new pair from PyTorch's generator of the device; while a graph is captured, as a tensor that each replay fills anew.
+Rng draw_rng(const at::Device &device) {
+    auto gen = at::cuda::detail::getDefaultCUDAGenerator(device.index());
+    at::PhiloxCudaState drawn;
+    {
+        std::lock_guard<std::mutex> lock(gen.mutex());
+        drawn = at::check_generator<at::CUDAGeneratorImpl>(gen)->philox_cuda_state(4);
+    }
+    if (!drawn.captured_) return {drawn.seed_.val, drawn.offset_.val, std::nullopt};
+    Tensor state = at::empty({2}, at::TensorOptions().dtype(at::kLong).device(device));
+    check(pcx_rng_state((const int64_t *)drawn.seed_.ptr, drawn.offset_.ptr, (int64_t)drawn.offset_intragraph_, state.data_ptr<int64_t>(), stream()));
+    return {0, 0, state};
+}
+
+// None: a new one.  A pair of numbers (taken modulo 2^64), or an int64 tensor of two on the device.
+Rng take_rng(const py::object &given, const Tensor &x, double p) {
+    require(p >= 0 && p <= 1, PyExc_ValueError, [&] { return "dropout probability has to be between 0 and 1, but got " + std::to_string(p); });
+    if (given.is_none()) {
+        if (!(p > 0)) return {};
+        require_cuda(x);
+        c10::cuda::CUDAGuard guard(x.device());
+        return draw_rng(x.device());
+    }
+    if (THPVariable_Check(given.ptr())) {
+        const Tensor state = py::cast<Tensor>(given);
+        require(state.scalar_type() == at::kLong && state.numel() == 2 && state.is_contiguous() && state.device() == x.device(), PyExc_ValueError,
+                [] { return std::string("rng as a tensor has two int64, on the device of x"); });
+        return {0, 0, state};
+    }
+    require(PySequence_Check(given.ptr()) && PySequence_Size(given.ptr()) == 2, PyExc_TypeError,
+            [] { return std::string("rng is None, a pair (seed, offset) or an int64 tensor of the two"); });
+    Rng rng;
+    uint64_t *to[2] = {&rng.seed, &rng.offset};
+    for (int q = 0; q < 2; ++q) {
+        const py::object item = py::reinterpret_steal<py::object>(PySequence_GetItem(given.ptr(), q));
+        const py::object index = item ? py::reinterpret_steal<py::object>(PyNumber_Index(item.ptr())) : py::object();
+        if (!index) throw py::error_already_set();
+        *to[q] = (uint64_t)PyLong_AsUnsignedLongLongMask(index.ptr());
+    }
+    return rng;
+}
+
+py::object draw_rng_for(const Tensor &like) {
+    require_cuda(like);
+    c10::cuda::CUDAGuard guard(like.device());
+    const Rng rng = draw_rng(like.device());
+    if (rng.state) return py::cast(*rng.state);
+    return py::make_tuple(rng.seed, rng.offset);
+}
+
+void require_rows(const Tensor &x) {
+    require(x.dim() == 2, PyExc_ValueError, [&] { return "expected rows (points, channels), got " + str(x.sizes()); });
+}
+void require_like(const char *name, const OptTensor &t, const Tensor &x, at::IntArrayRef sizes) {
+    if (!t) return;
+    require_cuda(*t);
+    require(t->sizes() == sizes, PyExc_ValueError, [&] { return std::string(name) + " has the sizes " + str(t->sizes()) + ", expected " + str(sizes); });
+    require(t->device() == x.device(), PyExc_RuntimeError, [&] { return std::string(name) + " is on " + t->device().str() + ", x on " + x.device().str(); });
+}
+Tensor sample_lengths(const Tensor &lengths, const Tensor &x) {
+    require_cuda(lengths);
+    require(lengths.dim() == 1 && lengths.numel() > 0 && !lengths.is_floating_point() && lengths.device() == x.device(), PyExc_ValueError,
+            [] { return std::string("lengths are the rows of each sample: whole numbers, on the device of x"); });
+    return as_i64(lengths);
+}
+bool under_transforms() { return c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::FuncTorchDynamicLayerFrontMode); }
+bool differentiates(const OptTensor &t) { return t && ((at::GradMode::is_enabled() && t->requires_grad()) || t->_fw_grad(0).defined()); }
+
+// ----------------------------------- group norm, activation and dropout (autograd) ----
+struct Tail {   // what follows the norm
+    int64_t groups, activation;
+    double eps, dropout;
+    uint64_t seed, offset;
+};
+
+std::tuple<Tensor, Tensor, Tensor> group_norm_act_forward(Tensor x, const Tensor &lengths_, const OptTensor &weight_, const OptTensor &bias_,
+                                                          const OptTensor &residual_, const OptTensor &state, const Tail &t) {
+    require_rows(x);
+    require_cuda(x);
+    const int code = dtype_code(x.scalar_type());
+    c10::cuda::CUDAGuard guard(x.device());
+    const int64_t N = x.size(0), C = x.size(1);
+    require_like("weight", weight_, x, {C}), require_like("bias", bias_, x, {C}), require_like("residual", residual_, x, x.sizes());
+    require(t.groups > 0 && t.groups <= C && C % t.groups == 0, PyExc_ValueError,
+            [&] { return std::to_string(C) + " channels do not make " + std::to_string(t.groups) + " groups"; });
+    const Tensor lengths = sample_lengths(lengths_, x), weight = f32_or_none(weight_), bias = f32_or_none(bias_);
+    x = x.contiguous();
+    const Tensor residual = residual_ ? residual_->to(x.scalar_type()).contiguous() : Tensor();
+    const int64_t S = lengths.numel();
+    Tensor y = at::empty_like(x);
+    Tensor stats = at::empty({2, S * t.groups}, x.options().dtype(at::kFloat));
+    Tensor mean = stats.select(0, 0), rstd = stats.select(0, 1);
+    Tensor ws = workspace(pcx_ragged_group_norm_act_workspace_bytes(N, S, (int)C, (int)t.groups, code), x);
+    check(pcx_ragged_group_norm_act(ptr(x), ptr_as<int64_t>(lengths), ptr_as<float>(weight), ptr_as<float>(bias), ptr(residual), ptr(y),
+                                    ptr_as<float>(mean), ptr_as<float>(rstd), N, S, (int)C, (int)t.groups, t.eps, (int)t.activation, t.dropout, t.seed,
+                                    t.offset, state ? ptr_as<int64_t>(*state) : nullptr, code, ptr(ws), ws.numel(), stream()));
+    return {y, mean, rstd};
+}
+
+struct GroupNormAct : public torch::autograd::Function<GroupNormAct> {
+    static Tensor forward(torch::autograd::AutogradContext *ctx, const Tensor &x, const Tensor &lengths, const OptTensor &weight, const OptTensor &bias,
+                          const OptTensor &residual, const OptTensor &state, int64_t groups, double eps, int64_t activation, double dropout,
+                          int64_t seed, int64_t offset) {
+        auto [y, mean, rstd] =
+            group_norm_act_forward(x, lengths, weight, bias, residual, state, {groups, activation, eps, dropout, (uint64_t)seed, (uint64_t)offset});
+        const auto or_none = [](const OptTensor &t) { return t ? *t : Tensor(); };
+        ctx->save_for_backward({x, lengths, or_none(weight), or_none(bias), or_none(residual), or_none(state), mean, rstd});
+        // edges of the node exist for the tensors that were given: remember where theirs are (-1: none)
+        int64_t at = 2;
+        std::vector<int64_t> edges;
+        for (const OptTensor *t : {&weight, &bias, &residual}) edges.push_back(*t ? at++ : -1);
+        ctx->saved_data["edges"] = edges;
+        ctx->saved_data["sizes"] = std::vector<int64_t>{groups, activation, seed, offset};
+        ctx->saved_data["dropout"] = dropout;
+        return y;
+    }
+
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list grads) {
+        const auto saved = ctx->get_saved_variables();
+        torch::autograd::variable_list out(12);
+        if (!grads[0].defined()) return out;
+        at::AutoGradMode no_graph(false);   // once differentiable, as the ragged layer norm
+        const auto edges = ctx->saved_data["edges"].toIntVector(), sizes = ctx->saved_data["sizes"].toIntVector();
+        const auto needs = [&](int q) { return edges[q] >= 0 && ctx->needs_input_grad((size_t)edges[q]); };
+        const auto given = [](const Tensor &t) { return t.defined() ? OptTensor(t) : std::nullopt; };
+        const Tensor x = saved[0].contiguous(), grad_y = grads[0].contiguous();
+        c10::cuda::CUDAGuard guard(x.device());
+        const Tensor lengths = as_i64(saved[1]), weight = f32_or_none(given(saved[2])), bias = f32_or_none(given(saved[3]));
+        const Tensor residual = saved[4].defined() ? saved[4].to(x.scalar_type()).contiguous() : Tensor();
+        const int64_t N = x.size(0), C = x.size(1), S = lengths.numel();
+        const int code = dtype_code(x.scalar_type());
+        Tensor gx = at::empty_like(x), gaffine, gw, gb, gres;
+        if (needs(0) || needs(1)) {
+            gaffine = at::empty({2, C}, x.options().dtype(at::kFloat));
+            gw = gaffine.select(0, 0), gb = gaffine.select(0, 1);
+        }
+        if (needs(2)) gres = at::empty_like(x);
+        Tensor ws = workspace(pcx_ragged_group_norm_act_workspace_bytes(N, S, (int)C, (int)sizes[0], code), x);
+        check(pcx_ragged_group_norm_act_backward(ptr(grad_y), ptr(x), ptr(residual), ptr_as<int64_t>(lengths), ptr_as<float>(weight),
+                                                 ptr_as<float>(bias), ptr_as<float>(saved[6]), ptr_as<float>(saved[7]), ptr(gx), ptr_as<float>(gw),
+                                                 ptr_as<float>(gb), ptr(gres), N, S, (int)C, (int)sizes[0], (int)sizes[1],
+                                                 ctx->saved_data["dropout"].toDouble(), (uint64_t)sizes[2], (uint64_t)sizes[3],
+                                                 ptr_as<int64_t>(saved[5]), code, ptr(ws), ws.numel(), stream()));
+        out[0] = gx;
+        if (gw.defined()) out[2] = gw.to(saved[2].scalar_type()), out[3] = gb.to(saved[3].scalar_type());
+        if (gres.defined()) out[4] = gres.to(saved[4].scalar_type());
+        return out;
+    }
+};
+
+Tensor group_norm_act(const Tensor &x, const Tensor &lengths, int64_t groups, const OptTensor &weight, const OptTensor &bias, double eps,
+                      const OptTensor &residual, int64_t activation, double dropout, const py::object &rng_) {
+    const Rng rng = take_rng(rng_, x, dropout);
+    if (!under_transforms() && !differentiates(x) && !differentiates(weight) && !differentiates(bias) && !differentiates(residual))
+        return std::get<0>(group_norm_act_forward(x, lengths, weight, bias, residual, rng.state, {groups, activation, eps, dropout, rng.seed, rng.offset}));
+    return GroupNormAct::apply(x, lengths, weight, bias, residual, rng.state, groups, eps, activation, dropout, (int64_t)rng.seed, (int64_t)rng.offset);
+}
+
+// -------------------------------------------------------------- dropout (autograd) ----
+struct DropShape {   // rows and channels of x; by element it may have any shape
+    int64_t N, C;
+};
+DropShape drop_shape(const Tensor &x, int64_t unit) {
+    if (unit != PCX_DROP_ELEMENT) {
+        require_rows(x);
+        return {x.size(0), x.size(1)};
+    }
+    return {x.numel(), 1};
+}
+
+Tensor dropout_forward(Tensor x, const OptTensor &lengths_, const OptTensor &residual_, const OptTensor &state, int64_t unit, bool relu, double p,
+                       uint64_t seed, uint64_t offset) {
+    require_cuda(x);
+    const int code = dtype_code(x.scalar_type());
+    c10::cuda::CUDAGuard guard(x.device());
+    require_like("residual", residual_, x, x.sizes());
+    require(unit == PCX_DROP_ELEMENT || lengths_.has_value(), PyExc_ValueError, [] { return std::string("lengths are needed to drop channels or samples"); });
+    const auto [N, C] = drop_shape(x, unit);
+    const Tensor lengths = unit == PCX_DROP_ELEMENT ? Tensor() : sample_lengths(*lengths_, x);
+    x = x.contiguous();
+    const Tensor residual = residual_ ? residual_->to(x.scalar_type()).contiguous() : Tensor();
+    const int64_t S = lengths.defined() ? lengths.numel() : 0;
+    Tensor y = at::empty_like(x), ws;
+    if (lengths.defined()) ws = workspace(pcx_dropout_workspace_bytes(S, (int)unit), x);
+    if (x.numel())
+        check(pcx_dropout(ptr(x), ptr_as<int64_t>(lengths), ptr(residual), ptr(y), N, S, (int)C, (int)unit, relu, p, seed, offset,
+                          state ? ptr_as<int64_t>(*state) : nullptr, code, ptr(ws), ws.defined() ? ws.numel() : 0, stream()));
+    return y;
+}
+
+Tensor dropout_with(const Tensor &x, const OptTensor &lengths, const OptTensor &residual, const OptTensor &state, int64_t unit, bool relu, double p,
+                    int64_t seed, int64_t offset);
+
+struct Dropout : public torch::autograd::Function<Dropout> {
+    static Tensor forward(torch::autograd::AutogradContext *ctx, const Tensor &x, const OptTensor &lengths, const OptTensor &residual,
+                          const OptTensor &state, int64_t unit, bool relu, double p, int64_t seed, int64_t offset) {
+        Tensor y = dropout_forward(x, lengths, residual, state, unit, relu, p, (uint64_t)seed, (uint64_t)offset);
+        const auto or_none = [](const OptTensor &t) { return t ? *t : Tensor(); };
+        ctx->save_for_backward({relu ? y : Tensor(), or_none(lengths), or_none(state)});
+        ctx->saved_data["sizes"] = std::vector<int64_t>{unit, relu, seed, offset, residual ? (lengths ? 2 : 1) : -1};
+        ctx->saved_data["p"] = p;
+        ctx->saved_data["residual_type"] = (int64_t)(residual ? residual->scalar_type() : x.scalar_type());
+        return y;
+    }
+
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list grads) {
+        const auto saved = ctx->get_saved_variables();
+        torch::autograd::variable_list out(9);
+        if (!grads[0].defined()) return out;
+        const auto sizes = ctx->saved_data["sizes"].toIntVector();
+        const int64_t unit = sizes[0];
+        const double p = ctx->saved_data["p"].toDouble();
+        const bool relu = sizes[1], want_x = ctx->needs_input_grad(0), want_res = sizes[4] >= 0 && ctx->needs_input_grad((size_t)sizes[4]);
+        const auto res_type = (at::ScalarType)ctx->saved_data["residual_type"].toInt();
+        const auto given = [](const Tensor &t) { return t.defined() ? OptTensor(t) : std::nullopt; };
+        if (!relu || at::GradMode::is_enabled()) {   // (the operator again: linear, and differentiable as often as asked for)
+            const Tensor g = relu ? grads[0] * (saved[0].detach() > 0) : grads[0];
+            if (want_x) out[0] = dropout_with(g, given(saved[1]), std::nullopt, given(saved[2]), unit, false, p, sizes[2], sizes[3]);
+            if (want_res) out[2] = g.to(res_type);
+            return out;
+        }
+        const Tensor g = grads[0].contiguous(), y = saved[0];
+        c10::cuda::CUDAGuard guard(g.device());
+        const auto [N, C] = drop_shape(g, unit);
+        const Tensor lengths = unit == PCX_DROP_ELEMENT ? Tensor() : as_i64(saved[1]);
+        const int64_t S = lengths.defined() ? lengths.numel() : 0;
+        Tensor gx = at::empty_like(g), gres, ws;
+        if (want_res) gres = at::empty_like(g);
+        if (lengths.defined()) ws = workspace(pcx_dropout_workspace_bytes(S, (int)unit), g);
+        if (g.numel())
+            check(pcx_dropout_backward(ptr(g), ptr(y), ptr_as<int64_t>(lengths), ptr(gx), ptr(gres), N, S, (int)C, (int)unit, relu, p,
+                                       (uint64_t)sizes[2], (uint64_t)sizes[3], ptr_as<int64_t>(saved[2]), dtype_code(g.scalar_type()), ptr(ws),
+                                       ws.defined() ? ws.numel() : 0, stream()));
+        if (want_x) out[0] = gx;
+        if (want_res) out[2] = gres.to(res_type);
+        return out;
+    }
+};
+
+Tensor dropout_with(const Tensor &x, const OptTensor &lengths, const OptTensor &residual, const OptTensor &state, int64_t unit, bool relu, double p,
+                    int64_t seed, int64_t offset) {
+    if (!under_transforms() && !differentiates(x) && !differentiates(residual))
+        return dropout_forward(x, lengths, residual, state, unit, relu, p, (uint64_t)seed, (uint64_t)offset);
+    return Dropout::apply(x, lengths, residual, state, unit, relu, p, seed, offset);
+}
+
+Tensor dropout(const Tensor &x, double p, const py::object &rng_, int64_t unit, const OptTensor &lengths, const OptTensor &residual, bool relu) {
+    const Rng rng = take_rng(rng_, x, p);
+    return dropout_with(x, lengths, residual, rng.state, unit, relu, p, (int64_t)rng.seed, (int64_t)rng.offset);
+}
+
 // ----------------------------------------------------------------- geometry ----
 // Sample ids as the searches and the down-sampling read them: 64-bit ones by their low words, where they lie.
 Tensor ids(const Tensor &t) { return t.scalar_type() == at::kLong ? t.contiguous() : as_i32(t); }
@@ -740,6 +999,9 @@ PYBIND11_MODULE(_pcx_host, m) {
           py::arg("n_in"), py::arg("K"), py::arg("cover_out"), py::arg("cover_in"), py::arg("plan_padded") = false);
     m.def("column_sums", &column_sums);
     m.def("layer_norm", &layer_norm);
+    m.def("group_norm_act", &group_norm_act);
+    m.def("dropout", &dropout);
+    m.def("draw_rng", &draw_rng_for);
     m.def("radius_taps", &radius_taps, py::call_guard<py::gil_scoped_release>());
     m.def("grid_sample", &grid_sample, py::call_guard<py::gil_scoped_release>());
     m.def("peek", &peek);

@@ -2,6 +2,8 @@
 // 16-byte vector loads / stores of VN consecutive channels converted to fp32, and
 // the thread layout (vector column, row lane) they share.
 #pragma once
+#include <initializer_list>
+
 #include "common.cuh"
 
 namespace pcx {
@@ -68,5 +70,66 @@ static inline bool vec_ok(int C, int dtype, std::initializer_list<const void *> 
         if (p && ((uintptr_t)p & 15)) return false;
     return true;
 }
+
+// VN consecutive channels as they lie in memory: accesses of at most 16 bytes.
+template <typename T, int VN>
+struct Lump {
+    static constexpr int BYTES = VN * (int)sizeof(T);
+    static constexpr int WORDS = (BYTES + 3) / 4;
+    uint32_t w[WORDS];
+    __device__ __forceinline__ void load(const T *__restrict__ p) {
+        if constexpr (BYTES >= 16) {
+#pragma unroll
+            for (int q = 0; q < BYTES / 16; ++q) {
+                const uint4 v = reinterpret_cast<const uint4 *>(p)[q];
+                w[4 * q] = v.x, w[4 * q + 1] = v.y, w[4 * q + 2] = v.z, w[4 * q + 3] = v.w;
+            }
+        } else if constexpr (BYTES == 8) {
+            const uint2 v = *reinterpret_cast<const uint2 *>(p);
+            w[0] = v.x, w[1] = v.y;
+        } else if constexpr (BYTES == 4) {
+            w[0] = *reinterpret_cast<const uint32_t *>(p);
+        } else {
+            w[0] = *reinterpret_cast<const uint16_t *>(p);
+        }
+    }
+    __device__ __forceinline__ void store(T *__restrict__ p) const {
+        if constexpr (BYTES >= 16) {
+#pragma unroll
+            for (int q = 0; q < BYTES / 16; ++q) reinterpret_cast<uint4 *>(p)[q] = make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
+        } else if constexpr (BYTES == 8) {
+            *reinterpret_cast<uint2 *>(p) = make_uint2(w[0], w[1]);
+        } else if constexpr (BYTES == 4) {
+            *reinterpret_cast<uint32_t *>(p) = w[0];
+        } else {
+            *reinterpret_cast<uint16_t *>(p) = (uint16_t)w[0];
+        }
+    }
+    __device__ __forceinline__ float get(int i) const { return to_f32<T>(reinterpret_cast<const T *>(w)[i]); }
+    __device__ __forceinline__ void set(int i, float v) { reinterpret_cast<T *>(w)[i] = from_f32<T>(v); }
+};
+
+// max(v, 0) that hands a NaN on
+__device__ __forceinline__ float relu(float v) {
+    float out;
+    asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(out) : "f"(v));
+    return out;
+}
+
+// Channels of a lump: the most that divide a row and that the pointers are aligned for.
+static inline int lump_of(int C, int dtype, std::initializer_list<const void *> pointers) {
+    int vn = 8;
+    for (; vn > 1; vn /= 2) {
+        const uintptr_t align = vn * elem_size(dtype) < 16 ? vn * elem_size(dtype) : 16;
+        bool ok = C % vn == 0;
+        for (const void *q : pointers) ok = ok && (uintptr_t)q % align == 0;
+        if (ok) break;
+    }
+    return vn;
+}
+
+// Row offsets (S + 1) of a batch from its lengths: they ascend within 0 .. N whatever the lengths say, and rows behind the last
+// sample are its own.  (norm_act.cu)
+int sample_offsets(const int64_t *d_lengths, int64_t *offsets, int64_t S, int64_t N, cudaStream_t stream);
 
 }  // namespace pcx

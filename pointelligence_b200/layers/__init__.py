@@ -2,6 +2,7 @@ from .contract import TripletContract
 from .conv import (GeneralConv, GenerativePointConv3d, PointConv3d, conv_with_stride, conv_with_stride_disjoint,
                    conv_with_stride_full_cover)
 from .downsample import downsample
+from .dropout import RaggedDropout
 from .generative import (CoordinateGenerator, GeneratedSites, KernelStampGenerator, SubdivisionGenerator,
                          build_generative_triplets)
 from .metadata import MetaData
@@ -21,4 +22,4 @@ __all__ = ["TripletContract", "GeneralConv", "GenerativePointConv3d", "Coordinat
            "handle_stride_and_build_triplets", "minimum_full_cover_kernel_size",
            "radius_scaler_for_kernel_size", "should_use_direct_segmented_triplets", "voxelize_3d",
            "RaggedNorm", "RaggedBatchNorm", "RaggedInstanceNorm", "RaggedLayerNorm", "RaggedGroupNorm",
-           "GlobalPool", "max_pool3d"]
+           "RaggedDropout", "GlobalPool", "max_pool3d"]

@@ -21,7 +21,9 @@ from .. import _cabi
 from ..sparse_engines.segment_reduce import large_segment_reduce
 
 __all__ = ["RaggedNorm", "RaggedBatchNorm", "RaggedInstanceNorm", "RaggedLayerNorm", "RaggedGroupNorm",
-           "fused_layer_norm", "fused_group_norm"]
+           "fused_layer_norm", "fused_group_norm", "fused_group_norm_act"]
+
+ACTIVATIONS = {"identity": 0, "relu": 1, "silu": 2, "gelu": 3}
 
 
 class _FusedGroupNorm(torch.autograd.Function):
@@ -58,6 +60,20 @@ def fused_layer_norm(x, lengths, weight=None, bias=None, eps=1e-5, residual=None
     Same arithmetic as ``RaggedLayerNorm`` (layers/norm.py:59-83,118-130 of the reference) followed by
     the ``out += identity; relu(out)`` tail of its residual blocks (models/resnet.py:129-130)."""
     return _cabi.host().layer_norm(x, lengths, weight, bias, residual, float(eps), bool(relu))
+
+
+def fused_group_norm_act(x, lengths, groups, weight=None, bias=None, eps=1e-5, residual=None, activation="silu", dropout=0.0, rng=None):
+    """``dropout(activation(group_norm(x) (+ residual)))`` per sample of a ragged batch, in the norm's own passes over the
+    rows (CUDA tensors only): x (points, channels), ``lengths`` rows per sample, ``groups`` blocks of consecutive channels (1: the
+    statistics of ``RaggedLayerNorm``, ``x.shape[1]``: of ``RaggedInstanceNorm``).
+
+    ``activation``: "identity", "relu", "silu" or "gelu" (the erf form).  ``dropout`` is the probability of dropping an
+    element; its mask follows from ``rng`` as in ``layers.dropout.fused_dropout``, and is the one that call would take.  Nothing
+    but the statistics is kept for the backward pass, which makes the activation's argument and the mask again; the gradients'
+    sums are merged in a fixed order.  Differentiable once."""
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"activation is one of {sorted(ACTIVATIONS)}, got {activation!r}")
+    return _cabi.host().group_norm_act(x, lengths, groups, weight, bias, eps, residual, ACTIVATIONS[activation], dropout, rng)
 
 
 class RaggedNorm(nn.Module):
