@@ -15,7 +15,8 @@ namespace pcx {
 namespace {
 
 constexpr int DO_THREADS = 256;
-constexpr int DO_UNROLL = 4;                  // lumps a thread has in flight
+constexpr int DO_UNROLL = 4;                  // lumps a thread has in flight (by channel or sample)
+constexpr int DO_CALLS = 2;                   // of the generator, a thread (by element)
 constexpr int DO_CHUNK_BYTES = 16 << 10;      // of rows, a block of the units' kernel
 
 struct DropArgs {
@@ -27,22 +28,25 @@ struct DropArgs {
     Dropping drop;
 };
 
+// `words`: of the lump's units; all ones: kept.
+__device__ __forceinline__ bool is_kept(const DropArgs &p, const uint32_t *words, int i) { return (i % 2 ? words[i / 2] : words[i / 2] << 16) > p.drop.over; }
+
 template <typename T, int VN, bool BACKWARD>
-__device__ __forceinline__ void drop_lump(const DropArgs &p, int64_t at, const Lump<T, VN> &x, const Lump<T, VN> &other, const float *factor) {
+__device__ __forceinline__ void drop_lump(const DropArgs &p, int64_t at, const Lump<T, VN> &x, const Lump<T, VN> &other, const uint32_t *words) {
     Lump<T, VN> out;
     if constexpr (BACKWARD) {
-        Lump<T, VN> g;
+        Lump<T, VN> g = x;
+        if (p.relu) {
 #pragma unroll
-        for (int i = 0; i < VN; ++i) {
-            const float v = p.relu && !(other.get(i) > 0.f) ? 0.f : x.get(i);
-            g.set(i, v);
-            out.set(i, factor[i] > 0.f ? v * factor[i] : 0.f);
+            for (int i = 0; i < VN; ++i) g.set(i, other.get(i) > 0.f ? x.get(i) : 0.f);
         }
+#pragma unroll
+        for (int i = 0; i < VN; ++i) out.set(i, is_kept(p, words, i) ? g.get(i) * p.drop.scale : 0.f);
         if (p.masked) g.store(static_cast<T *>(p.masked) + at);
     } else {
 #pragma unroll
         for (int i = 0; i < VN; ++i) {
-            float v = factor[i] > 0.f ? x.get(i) * factor[i] : 0.f;
+            float v = is_kept(p, words, i) ? x.get(i) * p.drop.scale : 0.f;
             if (p.residual) v += other.get(i);
             out.set(i, p.relu ? relu(v) : v);
         }
@@ -50,48 +54,62 @@ __device__ __forceinline__ void drop_lump(const DropArgs &p, int64_t at, const L
     out.store(static_cast<T *>(p.y) + at);
 }
 
-// By element: a thread takes groups of eight consecutive ones, with the words of one call.
-// VN = 8: accesses of 16 bytes; 1: of one element, for tensors at other addresses.
-template <typename T, int VN, bool BACKWARD>
-__global__ void __launch_bounds__(DO_THREADS) drop_elements_kernel(const __grid_constant__ DropArgs p, int64_t n) {
+// By element: a thread takes groups of eight consecutive ones, with the words of one call.  PLAIN: nothing but the dropout; WIDE: accesses
+// of 16 bytes (addresses are multiples of that).
+template <typename T, bool WIDE, bool STATE, bool PLAIN, bool BACKWARD>
+__global__ void __launch_bounds__(DO_THREADS, 6) drop_elements_kernel(const __grid_constant__ DropArgs p, int64_t n) {
     start_after_previous();
-    const Philox rng(p.drop);
+    const Philox<STATE> rng(p.drop);
     const T *x = static_cast<const T *>(p.x), *other = static_cast<const T *>(BACKWARD ? p.y_in : p.residual);
-    const bool reads = BACKWARD ? p.relu != 0 : p.residual != nullptr;
-    const int64_t g0 = (int64_t)blockIdx.x * (DO_THREADS * DO_UNROLL) + threadIdx.x;
-    if constexpr (VN == 8) {
-        Lump<T, 8> v[DO_UNROLL], q[DO_UNROLL];
+    const bool reads = !PLAIN && (BACKWARD ? p.relu != 0 : p.residual != nullptr);
+    const int64_t call0 = (int64_t)blockIdx.x * (DO_THREADS * DO_CALLS) + threadIdx.x;
+    uint32_t words[DO_CALLS][4];
+    if (WIDE && ((int64_t)blockIdx.x + 1) * (DO_THREADS * DO_CALLS * 8) <= n) {
+        Lump<T, 8> v[DO_CALLS], q[DO_CALLS];
+        x += call0 * 8;
+        if (reads) other += call0 * 8;
 #pragma unroll
-        for (int u = 0; u < DO_UNROLL; ++u) {
-            const int64_t at = (g0 + u * DO_THREADS) * 8;
-            if (at + 8 <= n) {
-                v[u].load(x + at);
-                if (reads) q[u].load(other + at);
+        for (int u = 0; u < DO_CALLS; ++u) {
+            v[u].load(x + u * DO_THREADS * 8);
+            if (reads) q[u].load(other + u * DO_THREADS * 8);
+        }
+#pragma unroll
+        for (int u = 0; u < DO_CALLS; ++u) {   // (while the loads are on their way)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) words[u][j] = ~0u;
+            if (PLAIN || p.drop.on) rng.template words<8>((uint64_t)(call0 + u * DO_THREADS) * 8, words[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < DO_CALLS; ++u) {
+            if constexpr (PLAIN) {
+                T *y = static_cast<T *>(p.y) + call0 * 8;
+                Lump<T, 8> out;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float2 f = mul2(pair_of(v[u], j), both(p.drop.scale));
+                    set_pair(out, j, make_float2((words[u][j] << 16) > p.drop.over ? f.x : 0.f, words[u][j] > p.drop.over ? f.y : 0.f));
+                }
+                out.store(y + u * DO_THREADS * 8);
+            } else {
+                drop_lump<T, 8, BACKWARD>(p, (call0 + u * DO_THREADS) * 8, v[u], q[u], words[u]);
             }
         }
-#pragma unroll
-        for (int u = 0; u < DO_UNROLL; ++u) {
-            const int64_t at = (g0 + u * DO_THREADS) * 8;
-            if (at + 8 > n) break;
-            const uint32_t kept = p.drop.on ? rng.kept<8>((uint64_t)at, p.drop.over) : 0xff;
-            float f[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) f[i] = kept >> i & 1 ? p.drop.scale : 0.f;
-            drop_lump<T, 8, BACKWARD>(p, at, v[u], q[u], f);
-        }
+        return;
     }
-    for (int u = 0; u < DO_UNROLL; ++u) {   // one by one: all of them, or the last group's
-        const int64_t from = (g0 + u * DO_THREADS) * 8;
+    for (int u = 0; u < DO_CALLS; ++u) {   // one by one
+        const int64_t from = (call0 + u * DO_THREADS) * 8;
         if (from >= n) break;
-        if (VN == 8 && from + 8 <= n) continue;
-        const uint32_t kept = p.drop.on ? rng.kept<8>((uint64_t)from, p.drop.over) : 0xff;
+        words[0][0] = words[0][1] = words[0][2] = words[0][3] = ~0u;
+        if (p.drop.on) rng.template words<8>((uint64_t)from, words[0]);
         const int count = (int)min(n - from, (int64_t)8);
-        for (int i = 0; i < count; ++i) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if (i >= count) break;
             Lump<T, 1> v, q;
             v.load(x + from + i);
             if (reads) q.load(other + from + i);
-            const float f = kept >> i & 1 ? p.drop.scale : 0.f;
-            drop_lump<T, 1, BACKWARD>(p, from + i, v, q, &f);
+            const uint32_t word = words[0][i / 2] >> 16 * (i & 1);
+            drop_lump<T, 1, BACKWARD>(p, from + i, v, q, &word);
         }
     }
 }
@@ -100,7 +118,7 @@ __global__ void __launch_bounds__(DO_THREADS) drop_elements_kernel(const __grid_
 template <typename T, int VN, bool BACKWARD, bool SAMPLES>
 __global__ void __launch_bounds__(DO_THREADS) drop_units_kernel(const __grid_constant__ DropArgs p) {
     start_after_previous();
-    const Philox rng(p.drop);
+    const Philox<true> rng(p.drop);
     const T *x = static_cast<const T *>(p.x), *other = static_cast<const T *>(BACKWARD ? p.y_in : p.residual);
     const bool reads = BACKWARD ? p.relu != 0 : p.residual != nullptr;
     const int lumps = p.C / VN, cols = min(lumps, DO_THREADS), lanes = DO_THREADS / cols, col = threadIdx.x % cols, lane = threadIdx.x / cols;
@@ -109,15 +127,21 @@ __global__ void __launch_bounds__(DO_THREADS) drop_units_kernel(const __grid_con
     for (int64_t s = segment_of_row(p.offsets, p.S, row0); s < p.S && p.offsets[s] < row1; ++s) {
         const int64_t lo = max(row0, p.offsets[s]), hi = min(row1, p.offsets[s + 1]);
         if (hi <= lo) continue;
-        uint32_t kept = 0xff;
-        if (SAMPLES && p.drop.on) kept = rng.kept<1>((uint64_t)s, p.drop.over) ? 0xff : 0;
+        uint32_t words[(VN + 1) / 2];
+#pragma unroll
+        for (int j = 0; j < (VN + 1) / 2; ++j) words[j] = ~0u;
+        if (SAMPLES && p.drop.on) {
+            rng.words<1>((uint64_t)s, words);
+            words[0] = (words[0] & 0xffff) * 0x10001;   // the sample's, for all
+#pragma unroll
+            for (int j = 1; j < (VN + 1) / 2; ++j) words[j] = words[0];
+        }
         for (int lump = col; lump < lumps; lump += cols) {
             const int c0 = lump * VN;
-            if (!SAMPLES && p.drop.on) kept = rng.kept<VN>((uint64_t)s * p.C + c0, p.drop.over);
-            const bool want = kept || (BACKWARD && p.masked);
-            float f[VN];
+            if (!SAMPLES && p.drop.on) rng.words<VN>((uint64_t)s * p.C + c0, words);
+            bool want = BACKWARD && p.masked;
 #pragma unroll
-            for (int i = 0; i < VN; ++i) f[i] = kept >> i & 1 ? p.drop.scale : 0.f;
+            for (int i = 0; i < VN; ++i) want |= is_kept(p, words, i);
             for (int64_t r = lo + lane; r < hi; r += (int64_t)DO_UNROLL * lanes) {
                 Lump<T, VN> v[DO_UNROLL], q[DO_UNROLL];
 #pragma unroll
@@ -133,7 +157,7 @@ __global__ void __launch_bounds__(DO_THREADS) drop_units_kernel(const __grid_con
 #pragma unroll
                 for (int u = 0; u < DO_UNROLL; ++u) {
                     const int64_t row = r + (int64_t)u * lanes;
-                    if (row < hi) drop_lump<T, VN, BACKWARD>(p, row * p.C + c0, v[u], q[u], f);
+                    if (row < hi) drop_lump<T, VN, BACKWARD>(p, row * p.C + c0, v[u], q[u], words);
                 }
             }
         }
@@ -142,11 +166,11 @@ __global__ void __launch_bounds__(DO_THREADS) drop_units_kernel(const __grid_con
 
 enum { UNIT_ELEMENT = 0, UNIT_CHANNEL = 1, UNIT_SAMPLE = 2 };
 
-template <typename T, bool BACKWARD>
-int run_elements(const DropArgs &p, bool wide, int64_t n, cudaStream_t stream) {
-    const unsigned grid = (unsigned)((n + 8 * DO_THREADS * DO_UNROLL - 1) / (8 * DO_THREADS * DO_UNROLL));
-    if (wide) launch_after(drop_elements_kernel<T, 8, BACKWARD>, grid, DO_THREADS, 0, stream, p, n);
-    else launch_after(drop_elements_kernel<T, 1, BACKWARD>, grid, DO_THREADS, 0, stream, p, n);
+template <typename T, bool WIDE, bool STATE, bool BACKWARD>
+int run_elements(const DropArgs &p, int64_t n, cudaStream_t stream) {
+    const unsigned grid = (unsigned)((n + 8 * DO_THREADS * DO_CALLS - 1) / (8 * DO_THREADS * DO_CALLS));
+    if (!BACKWARD && WIDE && p.drop.on && !p.residual && !p.relu) launch_after(drop_elements_kernel<T, WIDE, STATE, true, BACKWARD>, grid, DO_THREADS, 0, stream, p, n);
+    else launch_after(drop_elements_kernel<T, WIDE, STATE, false, BACKWARD>, grid, DO_THREADS, 0, stream, p, n);
     PCX_LAUNCH_CHECK();
     return PCX_OK;
 }
@@ -162,7 +186,11 @@ int run_units(const DropArgs &p, int unit, cudaStream_t stream) {
 
 template <typename T, bool BACKWARD>
 int run(const DropArgs &p, int unit, int vn, cudaStream_t stream) {
-    if (unit == UNIT_ELEMENT) return run_elements<T, BACKWARD>(p, vn == 8, p.N * p.C, stream);
+    if (unit == UNIT_ELEMENT) {
+        const int64_t n = p.N * p.C;
+        if (vn < 8) return run_elements<T, false, true, BACKWARD>(p, n, stream);
+        return p.drop.state ? run_elements<T, true, true, BACKWARD>(p, n, stream) : run_elements<T, true, false, BACKWARD>(p, n, stream);
+    }
     if (vn == 8) return run_units<T, 8, BACKWARD>(p, unit, stream);
     if (vn == 4) return run_units<T, 4, BACKWARD>(p, unit, stream);
     if (vn == 2) return run_units<T, 2, BACKWARD>(p, unit, stream);
@@ -178,7 +206,7 @@ size_t carve(void *ws, int64_t S, int unit, int64_t **offsets) {
 
 bool sizes_ok(int64_t N, int64_t S, int C, int unit, int dtype) {
     return N >= 0 && C > 0 && unit >= UNIT_ELEMENT && unit <= UNIT_SAMPLE && (unit == UNIT_ELEMENT || (S > 0 && S <= INT32_MAX)) &&
-           (dtype == PCX_F32 || dtype == PCX_F16 || dtype == PCX_BF16) && N <= INT64_MAX / 8 / C && N * C / (8 * DO_THREADS) < INT32_MAX;
+           (dtype == PCX_F32 || dtype == PCX_F16 || dtype == PCX_BF16) && N <= INT64_MAX / 8 / C && N * C / (8 * DO_THREADS * DO_CALLS) < INT32_MAX;
 }
 
 template <bool BACKWARD>

@@ -1,0 +1,1196 @@
+// Group normalisation over a ragged batch with what follows it in a residual block, in the norm's own passes:
+//
+//   y = drop(act((x - mean[s,g]) * rstd[s,g] * weight + bias (+ residual)))
+//
+// Rows are points, channels lie last.  mean and rstd are the statistics of the rows of sample s and the W = C / G consecutive
+// channels of group g (G = 1: the ragged layer norm, G = C: the instance norm); act is the identity, ReLU, SiLU or the
+// erf form of GELU; drop is the dropout of philox.cuh by element (y's row-major index).
+//
+// Backward, with z the activation's argument (made again from x, not stored), xh = (x - mean) * rstd and n = rows_s * W:
+//   gz = drop'(g) * act'(z),   dresidual = gz,   dbias[c] = sum over rows of gz,   dweight[c] = sum over rows of gz * xh,
+//   gh = gz * weight,   dx = rstd * (gh - sum_{s,g}(gh) / n - xh * sum_{s,g}(gh * xh) / n).
+//
+// Everything is held in fp32 between one read of an element and its one rounding.
+//
+// Both directions take two passes over the rows, with sums between them, in one launch (behind a small one that lays the samples
+// out).  A chunk is `rows` consecutive rows; a piece is what a chunk has of one sample, piece chunk + s (pieces are ordered, and
+// the next one has a higher chunk or a higher sample by one).  Blocks take tickets, in ascending order, one at a time:
+//   sums of a chunk  two floats per channel and piece, whatever the group's width, and from them two per group
+//   apply of a chunk the second pass, once the sums of its samples are there
+//   affine           dweight and dbias of some channels, once those of all samples are
+// A sample's records of groups are merged by every block that applies rows of it, for itself: one turn through the L2 from the last
+// piece to the first row, where one block that merges for all makes it two.  Where records are many (`window` pieces), the block that
+// brings the last piece of a window merges these first.  Who merges does not matter to the result: records are merged in a fixed
+// order, and no float is ever added by an atomic.  A ticket waits only for tickets before it, which blocks that run have taken, and
+// sums wait for nothing: there is no deadlock, however few blocks are resident at once (a stream with a part of the chip).
+// Tickets are ordered so that a sample is applied some chunks after its sums, in the hope that the wait for them is over by then.
+//
+// What is summed:
+//   forward   mean and sum of squares about it.  A block sums x - k and its square, k the channel's value in the piece's first row:
+//             as k is one of the n summed values, (k - mean)^2 is at most their sum of squares M2, and what cancels in
+//             sum (x - k)^2 - n (mean - k)^2 is at most (n + 1) M2: n + 1 roundings at worst, one where rows are alike.
+//   backward  gz and gz * xh.
+#pragma once
+#include <algorithm>
+#include <atomic>
+
+#include "philox.cuh"
+#include "rowwise.cuh"
+#include "tcgen05.cuh"   // (the clock and the limit of bounded waits)
+
+namespace pcx {
+
+constexpr int NA_THREADS = 256;
+constexpr unsigned NA_STATUS = 32u;   // of a wait that ran out
+constexpr int AFFINE_CHANNELS = 8;    // of a ticket
+enum { TICKET = 0, WINDOWS_DONE = 1, WINDOWS = 2, CONTROL_WORDS = 4 };
+enum { ACT_NONE = 0, ACT_RELU = 1, ACT_SILU = 2, ACT_GELU = 3 };
+
+// The chunks of a sample: b0 .. b1 have rows of it (b1 < b0: none), first .. next - 1 end in it, and these are applied from
+// ticket `at` on.
+struct Span { int b0, b1, first, next, at; };
+
+struct NormAct {
+    const void *x, *residual, *g;
+    void *y, *dx, *dresidual;
+    const float *weight, *bias;
+    float *mean, *rstd;            // (S, G)
+    float *dweight, *dbias;
+    int64_t *offsets;              // (S + 1)
+    Span *spans;                   // (S)
+    float2 *rec;                   // (pieces, C): mean and M2; or sums of gz and gz * xh
+    float2 *of_piece, *of_window;  // (pieces, G), (windows, G): the same of groups, the sums with the channels' weights
+    int *control;                  // the words above, then windows that each sample has, pieces that each window has
+    unsigned int *status;
+    int64_t N, S;
+    int C, G, W, rows, chunks, window, lag, act;
+    int tile_rows, sums_tile_rows, stages, stage_bytes;   // of the ring
+    uint32_t by_width;             // c / W = c * by_width >> 32 (c * W < 2^32); W = 1: c
+    float eps;
+    Dropping drop;
+};
+
+// One direction for rows of T (norm_act_*.cu); `vn` channels a lump.
+template <typename T>
+int norm_act_rows(const NormAct &p, int vn, bool backward, cudaStream_t stream);
+
+#ifdef __CUDACC__
+namespace {
+
+__device__ __forceinline__ int *sample_count(const NormAct &p) { return p.control + CONTROL_WORDS; }
+__device__ __forceinline__ int *window_count(const NormAct &p) { return sample_count(p) + p.S; }
+// Windows are `window` pieces of a sample; they are numbered as pieces are: first_window + its windows before.
+__host__ __device__ inline int64_t windows_in_all(int64_t chunks, int64_t S, int window) { return chunks / window + S + 1; }
+__device__ __forceinline__ int64_t first_window(const NormAct &p, const Span &v, int64_t s) { return v.b0 / p.window + s; }
+__device__ __forceinline__ int windows_of(const NormAct &p, const Span &v) { return (v.b1 - v.b0) / p.window + 1; }
+
+__device__ __forceinline__ int group_of(const NormAct &p, int c) { return p.W == 1 ? c : (int)__umulhi((uint32_t)c, p.by_width); }
+
+// ------------------------------------------------------------ activations ----
+__device__ __forceinline__ float ex2(float v) {
+    float e;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(v));
+    return e;
+}
+__device__ __forceinline__ float rcp(float v) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+// 1 / v of both, with one reciprocal: the special function units give 16 results a clock and SM, and with two exponentials and two
+// reciprocals a pair they, not the memory, would bound a pass over 16-bit rows.  v in 1 .. 2^62.
+__device__ __forceinline__ float2 rcp2(float2 v) { return mul2(both(rcp(v.x * v.y)), make_float2(v.y, v.x)); }
+
+// 1 / (1 + exp(-z)); below z = -43 it stays at 2^-62
+__device__ __forceinline__ float2 sigmoid2(float2 z) {
+    const float2 t = mul2(z, both(-1.4426950408889634f));
+    return rcp2(add2(both(1.f), make_float2(fminf(ex2(t.x), 0x1p62f), fminf(ex2(t.y), 0x1p62f))));
+}
+// The normal distribution's function and density, by formula 7.1.26 of Abramowitz and Stegun for erfc(|z| / sqrt 2) / 2 (off by at most
+// 7.5e-8, an ulp of fp32): one exponential serves both.
+__device__ __forceinline__ void normal2(float2 z, float2 &cdf, float2 &density) {
+    const float2 a = make_float2(fminf(fabsf(z.x), 0x1p30f), fminf(fabsf(z.y), 0x1p30f));
+    const float2 t = rcp2(fma2(a, both(0.3275911f * 0.70710678f), both(1.f)));
+    const float2 h = mul2(mul2(a, a), both(-0.5f * 1.4426950408889634f));
+    const float2 e = make_float2(ex2(h.x), ex2(h.y));   // exp(-z^2 / 2)
+    float2 q = fma2(t, both(0.5f * 1.061405429f), both(0.5f * -1.453152027f));
+    q = fma2(t, q, both(0.5f * 1.421413741f));
+    q = fma2(t, q, both(0.5f * -0.284496736f));
+    q = fma2(t, q, both(0.5f * 0.254829592f));
+    q = mul2(mul2(q, t), e);
+    const float2 p = add2(both(1.f), neg2(q));
+    cdf = make_float2(z.x < 0.f ? q.x : p.x, z.y < 0.f ? q.y : p.y);
+    density = mul2(e, both(0.39894228f));
+}
+
+__device__ __forceinline__ float2 act2(int act, float2 z) {
+    if (act == ACT_RELU) return make_float2(relu(z.x), relu(z.y));
+    if (act == ACT_SILU) return mul2(z, sigmoid2(z));
+    if (act == ACT_GELU) {
+        float2 cdf, density;
+        normal2(z, cdf, density);
+        return mul2(z, cdf);
+    }
+    return z;
+}
+// g times the slope at z
+__device__ __forceinline__ float2 act2_backward(int act, float2 z, float2 g) {
+    if (act == ACT_RELU) return make_float2(z.x > 0.f ? g.x : 0.f, z.y > 0.f ? g.y : 0.f);
+    if (act == ACT_SILU) {   // s (1 + z (1 - s)) = s + z s (1 - s)
+        const float2 s = sigmoid2(z), zs = mul2(z, s);
+        return mul2(g, add2(s, fma2(zs, neg2(s), zs)));
+    }
+    if (act == ACT_GELU) {
+        float2 cdf, density;
+        normal2(z, cdf, density);
+        return mul2(g, fma2(z, density, cdf));
+    }
+    return g;
+}
+
+// The last of `n` ascending values that `at(i)` gives which is not over `v`; -1 where all are.  A whole warp asks.
+template <typename At>
+__device__ __forceinline__ int64_t last_not_over(int64_t n, int64_t v, At at) {
+    const int lane = threadIdx.x & 31;
+    int64_t lo = 0, step = n;
+    do {
+        const int64_t end = min(n, lo + step);
+        step = (end - lo + 31) / 32;
+        const int64_t i = lo + lane * step;
+        const unsigned found = __ballot_sync(0xffffffffu, i < end && at(i) <= v);
+        if (!found) return lo - 1;   // (only before the first value)
+        lo += (31 - __clz(found)) * step;
+    } while (step > 1);
+    return lo;
+}
+
+// The chunk that a ticket is for; true: its sums.
+__device__ __forceinline__ bool take_ticket(const NormAct &p, int ticket, int *chunk) {
+    // the last sample that is applied from this ticket on or from one before: its chunks, or sums of a later chunk
+    const int64_t run = last_not_over(p.S, ticket, [&](int64_t s) { return (int64_t)p.spans[s].at; });
+    *chunk = ticket;
+    if (run < 0) return true;
+    const Span v = p.spans[run];
+    const bool sums = ticket - v.at >= v.next - v.first;
+    *chunk = sums ? ticket - v.next : v.next - 1 - (ticket - v.at);   // (backwards: what was read last is still in the L2)
+    return sums;
+}
+
+// ------------------------------------------------------------ columns ----
+// Channels of a block: passes of `cols` lumps side by side, `lanes` rows.
+struct Columns {
+    int lumps, cols, lanes, passes, col, lane;
+    __host__ __device__ __forceinline__ Columns(int C, int VN, int thread) {
+        lumps = C / VN;
+        passes = (lumps + NA_THREADS - 1) / NA_THREADS;
+        cols = (lumps + passes - 1) / passes;
+        lanes = NA_THREADS / cols;
+        col = thread % cols, lane = thread / cols;
+    }
+};
+
+// Barrier of the threads that work on rows (all but the ring's producer).
+__device__ __forceinline__ void sync_workers() { asm volatile("bar.sync 1, %0;" ::"n"(NA_THREADS) : "memory"); }
+__device__ __forceinline__ bool sync_workers_and(bool v) {
+    uint32_t all;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.and.pred q, 1, %2, p;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(all) : "r"((uint32_t)v), "n"(NA_THREADS) : "memory");
+    return all != 0;
+}
+
+// Records that follow one another: `count` of `unit` rows each, but for the first and the last.
+struct Records {
+    const float2 *at;
+    int count;
+    float first, unit, last, all;   // rows
+};
+// Rows lo .. hi by spans of `unit` rows, the first of which begins at `from`.
+__device__ __forceinline__ Records records_of(const float2 *at, int count, int64_t lo, int64_t hi, int64_t from, int64_t unit) {
+    return {at, count, (float)(min(hi, from + unit) - lo), (float)unit, (float)(hi - (from + (count - 1) * unit)), (float)(hi - lo)};
+}
+
+// Sums over records, of which a thread has some.  Forward, with d a record's mean less the first one's (so that their differences, not the means, are rounded; the first's own
+// is zero, whatever its rows): of d, d^2 and M2.  Backward: of both sums.
+template <bool BACKWARD>
+struct RecordSums {
+    static constexpr int AHEAD = 8;   // loads at once
+    float a = 0.f, b = 0.f, m2 = 0.f, k = 0.f;
+    __device__ __forceinline__ void add(const Records &r, int stride, int g, int q, int deep) {
+        const float2 *at = r.at + g;
+        if constexpr (!BACKWARD) k = __ldcg(at).x;
+        for (int i = q; i < r.count; i += AHEAD * deep) {
+            float2 v[AHEAD];
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u) v[u] = i + u * deep < r.count ? __ldcg(at + (int64_t)(i + u * deep) * stride) : make_float2(BACKWARD ? 0.f : k, 0.f);
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u) {
+                if constexpr (BACKWARD) {
+                    a += v[u].x, b += v[u].y;
+                } else {
+                    const float d = v[u].x - k;
+                    a += d, b += d * d, m2 += v[u].y;
+                }
+            }
+        }
+    }
+    // (mean, M2) of all rows, or the two sums; `each`: elements of a row
+    __device__ __forceinline__ float2 done(const Records &r, int stride, int g, float each) const {
+        if constexpr (BACKWARD) return make_float2(a, b);
+        const float d = __ldcg(r.at + (int64_t)(r.count - 1) * stride + g).x - k, less = r.unit - r.last;   // the last one's rows are fewer
+        const float sum = (r.unit * a - less * d) * each, squares = (r.unit * b - less * d * d) * each, off = sum / (r.all * each);
+        return make_float2(k + off, fmaxf(m2 + squares - sum * off, 0.f));
+    }
+};
+
+// What a second pass needs of the groups that channels c0 .. c1 - 1 are in, from the sample's records, into `stats` (shared memory) by all
+// workers: mean and rstd, or the backward's two means.  Every block does this for itself, with the sample's windows counted: a block
+// that did it for all would keep them waiting for one more turn through the L2.  Threads stand side by side on the groups and, where
+// there are fewer of them, in rows on the records.
+template <bool BACKWARD>
+__device__ __forceinline__ void merge_groups(const NormAct &p, const Records &r, int groups, float2 *stats, float4 *scratch) {
+    const float each = (float)p.W, inverse = 1.f / (r.all * each);
+    const int wide = min(groups, NA_THREADS), at = threadIdx.x % wide, q = threadIdx.x / wide;
+    const bool shuffles = wide < 32 && 32 % wide == 0;
+    int deep = NA_THREADS / wide;
+    for (int base = 0; base < groups; base += wide) {
+        const int g = base + at;
+        RecordSums<BACKWARD> sums;
+        if (g < groups && q < deep) sums.add(r, p.G, g, q, deep);
+        if (shuffles) {   // a warp's rows first; then its first row has them
+            for (int o = 16; o >= wide; o >>= 1) {
+                sums.a += __shfl_xor_sync(0xffffffffu, sums.a, o), sums.b += __shfl_xor_sync(0xffffffffu, sums.b, o);
+                if (!BACKWARD) sums.m2 += __shfl_xor_sync(0xffffffffu, sums.m2, o);
+            }
+        }
+        const int rows = shuffles ? NA_THREADS / 32 : deep, step = shuffles ? 32 : wide;
+        if (rows > 1) {
+            scratch[threadIdx.x] = make_float4(sums.a, sums.b, sums.m2, 0.f);
+            sync_workers();
+            if (q == 0)
+#pragma unroll 4
+                for (int i = 1; i < rows; ++i) {
+                    const float4 v = scratch[i * step + at];
+                    sums.a += v.x, sums.b += v.y, sums.m2 += v.z;
+                }
+        }
+        if (g < groups && q == 0) {
+            const float2 v = sums.done(r, p.G, g, each);
+            stats[g] = BACKWARD ? make_float2(v.x * inverse, v.y * inverse) : make_float2(v.x, 1.f / sqrtf(v.y * inverse + p.eps));
+        }
+        sync_workers();
+    }
+}
+
+// Waits until a word is what a block before has to make it; at most a second, then it is reported, and the answer is false.
+__device__ __forceinline__ bool wait_for(const int *word, int value, unsigned int *status) {
+    __shared__ int there;
+    sync_workers();
+    if (threadIdx.x == 0) {
+        int v = 0;
+        const uint64_t t0 = tc::global_timer_ns();
+        for (unsigned turn = 0;; ++turn) {
+            asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(word) : "memory");
+            if (v == value) break;
+            if (turn % 64 == 63 && tc::global_timer_ns() - t0 > tc::WAIT_LIMIT_NS) {
+                atomicOr(status, NA_STATUS);
+                break;
+            }
+        }
+        there = v == value;
+    }
+    sync_workers();
+    return there;
+}
+
+// What the rows of a sample are mapped by, per channel of a pass, in shared memory: floats k of a lump's quad h lie side by side over the
+// columns, so that a warp reads them without conflicts.  (In registers they were most of what a thread held: 24 to 40 floats.)
+// Forward z = x a + b, with the mean in b: that rounds z by 2^-24 of |mean| / deviation more, as the mean's own rounding does.  Backward
+// z = (x - mu) a + b, as sums of gz (x - mu) want the difference, and dx = gz a - m1 - (x - mu) m2.
+enum { K_A = 0, K_B = 1, K_MU = 2, K_M1 = 3, K_M2 = 4 };
+template <int VN>
+struct Constants {
+    static constexpr int QUAD = VN < 4 ? VN : 4, PAIRS = QUAD < 2 ? 1 : QUAD / 2, QUADS = VN / QUAD;
+    float *at;
+    float2 *stats;             // of the second pass: the groups'
+    float4 *scratch;           // an entry a thread
+    int64_t s = -1;            // whose they are
+    int pass = -1;
+    __device__ __forceinline__ void read(const Columns &l, int k, int h, float2 *out) const {
+        // (volatile: read where they are used, in every round of a loop; taken out of it, as compilers would, they are registers again)
+        const uint32_t q = tc::smem_u32(at + ((k * QUADS + h) * l.cols + l.col) * QUAD);
+        float2 &a = out[0], &b = out[PAIRS - 1];
+        if constexpr (QUAD == 4) asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(a.x), "=f"(a.y), "=f"(b.x), "=f"(b.y) : "r"(q) : "memory");
+        else if constexpr (QUAD == 2) asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(a.x), "=f"(a.y) : "r"(q) : "memory");
+        else asm volatile("ld.shared.f32 %0, [%1];" : "=f"(a.x) : "r"(q) : "memory");
+        if (QUAD == 1) a.y = 0.f;
+    }
+    __device__ __forceinline__ void read_all(const Columns &l, int k, float2 *out) const {
+#pragma unroll
+        for (int h = 0; h < QUADS; ++h) {
+            const float4 v = *reinterpret_cast<const float4 *>(at + ((k * QUADS + h) * l.cols + l.col) * 4);
+            out[2 * h] = make_float2(v.x, v.y), out[2 * h + 1] = make_float2(v.z, v.w);
+        }
+    }
+    // By all workers, once they have met.  `second`: of the second pass, for which the sample's records are waited for; false: in vain.
+    template <bool BACKWARD>
+    __device__ __forceinline__ bool load(const NormAct &p, const Columns &l, int64_t s_, int pass_, bool second) {
+        const int c0 = pass_ * l.cols * VN, c1 = min(p.C, c0 + l.cols * VN), g0 = group_of(p, c0);
+        float w = 1.f, bias = 0.f, mu = 0.f, rs = 0.f;   // of the thread's first channel: read before the wait
+        const auto known = [&](int c) {
+            if (p.weight) w = __ldg(p.weight + c), bias = __ldg(p.bias + c);
+            if (BACKWARD) mu = __ldg(p.mean + s_ * p.G + group_of(p, c)), rs = __ldg(p.rstd + s_ * p.G + group_of(p, c));
+        };
+        if (c0 + (int)threadIdx.x < c1) known(c0 + threadIdx.x);
+        if (second) {
+            const Span v = p.spans[s_];
+            const int windows = windows_of(p, v);
+            const Records r = records_of(p.of_window + first_window(p, v, s_) * p.G + g0, windows, p.offsets[s_], p.offsets[s_ + 1], (int64_t)v.b0 * p.rows, (int64_t)p.window * p.rows);
+            if (!wait_for(sample_count(p) + s_, windows, p.status)) return false;
+            merge_groups<BACKWARD>(p, r, group_of(p, c1 - 1) - g0 + 1, stats, scratch);
+        }
+        s = s_, pass = pass_;
+        const int stride = QUADS * l.cols * QUAD;
+        for (int t = threadIdx.x; t < c1 - c0; t += NA_THREADS) {
+            if (t >= NA_THREADS) known(c0 + t);
+            const int col = t / VN, i = t % VN;
+            const float2 m = second ? stats[group_of(p, c0 + t) - g0] : make_float2(0.f, 0.f);
+            if (!BACKWARD) mu = m.x, rs = m.y;
+            float *to = at + ((i / QUAD) * l.cols + col) * QUAD + i % QUAD;
+            to[K_A * stride] = rs * w, to[K_B * stride] = BACKWARD ? bias : fmaf(-mu, rs * w, bias);
+            if (BACKWARD) to[K_MU * stride] = -mu;
+            if (BACKWARD && second) to[K_M1 * stride] = -m.x * rs, to[K_M2 * stride] = -m.y * rs * rs;
+        }
+        sync_workers();
+        return true;
+    }
+    // The statistics that were merged, for the caller: the block that has the sample's first chunk.
+    __device__ __forceinline__ void put_stats(const NormAct &p, const Columns &l) const {
+        const int c0 = pass * l.cols * VN, c1 = min(p.C, c0 + l.cols * VN), g0 = group_of(p, c0), groups = group_of(p, c1 - 1) - g0 + 1;
+        for (int g = threadIdx.x; g < groups; g += NA_THREADS) p.mean[s * p.G + g0 + g] = stats[g].x, p.rstd[s * p.G + g0 + g] = stats[g].y;
+    }
+};
+
+// ------------------------------------------------------------ sums of a piece ----
+// Two sums per channel of a thread's rows, folded over the block's row lanes; `out(c, a, b)` for every channel.
+template <int VN, typename Out>
+__device__ __forceinline__ void fold_lanes(const Columns &l, int pass, const float2 *a, const float2 *b, float2 *fold, Out out) {
+    sync_workers();   // (the piece before has been read)
+#pragma unroll
+    for (int i = 0; i < VN; ++i)
+        fold[i * NA_THREADS + threadIdx.x] = i % 2 ? make_float2(a[i / 2].y, b[i / 2].y) : make_float2(a[i / 2].x, b[i / 2].x);
+    sync_workers();
+    for (int t = threadIdx.x; t < l.cols * VN; t += NA_THREADS) {
+        const int i = t / l.cols, col = t % l.cols, lump = pass * l.cols + col;
+        float sa = 0.f, sb = 0.f;
+#pragma unroll 8
+        for (int q = 0; q < l.lanes; ++q) {
+            const float2 v = fold[i * NA_THREADS + q * l.cols + col];
+            sa += v.x, sb += v.y;
+        }
+        if (lump < l.lumps) out(lump * VN + i, sa, sb);
+    }
+}
+
+// `U` rows of a thread's lumps, `lanes` apart; those behind the end are not read.  Rows are counted from the piece's first: a chunk's
+// elements fit 32 bits.
+template <typename T, int VN, int U>
+struct Rows {
+    Lump<T, VN> v[U];
+    __device__ __forceinline__ void load(const T *__restrict__ col, int r, int n, int lanes, int C) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (r + u * lanes < n) v[u].load(col + (r + u * lanes) * C);
+    }
+};
+
+template <typename T, int VN>
+__device__ __forceinline__ void stats_piece(const NormAct &p, const Columns &l, int64_t piece, int64_t lo, int n, float2 *fold) {
+    constexpr int U = sizeof(T) == 4 && VN == 8 ? 2 : 4, P = (VN + 1) / 2;
+    const T *x = static_cast<const T *>(p.x) + lo * p.C;
+    for (int pass = 0; pass < l.passes; ++pass) {
+        const int lump = pass * l.cols + l.col;
+        float2 a[P], b[P];
+#pragma unroll
+        for (int j = 0; j < P; ++j) a[j] = b[j] = both(0.f);
+        if (lump < l.lumps && l.lane < l.lanes) {
+            const T *col = x + (int64_t)lump * VN;
+            Lump<T, VN> first;
+            first.load(col);
+            int r = l.lane;
+            Rows<T, VN, U> in;
+            in.load(col, r, n, l.lanes, p.C);
+            float2 k[P];
+#pragma unroll
+            for (int j = 0; j < P; ++j) k[j] = neg2(pair_of(first, j));
+            for (; r < n; r += U * l.lanes) {
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    if (r + u * l.lanes < n)
+#pragma unroll
+                        for (int j = 0; j < P; ++j) {
+                            const float2 d = add2(pair_of(in.v[u], j), k[j]);
+                            a[j] = add2(a[j], d), b[j] = fma2(d, d, b[j]);
+                        }
+                in.load(col, r + U * l.lanes, n, l.lanes, p.C);
+            }
+        }
+        fold_lanes<VN>(l, pass, a, b, fold, [&](int c, float sa, float sb) {
+            const float off = sa / (float)n;
+            p.rec[piece * p.C + c] = make_float2(to_f32<T>(x[c]) + off, fmaxf(sb - sa * off, 0.f));
+        });
+    }
+}
+
+template <int VN>
+__device__ __forceinline__ float2 drop2(const NormAct &p, const uint32_t *words, int j, float2 v) {
+    v = mul2(v, both(p.drop.scale));
+    return make_float2((words[j] << 16) > p.drop.over ? v.x : 0.f, words[j] > p.drop.over ? v.y : 0.f);
+}
+
+// ------------------------------------------------------------ second pass, forward ----
+template <typename T, int VN, int ACT, int DROP>
+__device__ __forceinline__ bool apply_piece(const NormAct &p, const Columns &l, const Philox<DROP != 1> &rng, Constants<VN> &k, int64_t s, int64_t lo, int n, bool owner) {
+    constexpr int U = (sizeof(T) == 4 && VN == 8 ? 2 : 4) / (DROP ? 2 : 1), P = (VN + 1) / 2, PAIRS = Constants<VN>::PAIRS;
+    const int64_t from = lo * p.C;
+    const T *x = static_cast<const T *>(p.x) + from, *res = p.residual ? static_cast<const T *>(p.residual) + from : nullptr;
+    T *y = static_cast<T *>(p.y) + from;
+    const int act = ACT < 0 ? p.act : ACT;
+    const bool drop = DROP < 0 ? p.drop.on : DROP;
+    for (int pass = 0; pass < l.passes; ++pass) {
+        const int lump = pass * l.cols + l.col, c0 = lump * VN;
+        const bool mine = lump < l.lumps && l.lane < l.lanes;
+        int r = mine ? l.lane : n;
+        Rows<T, VN, U> v, q;
+        v.load(x + c0, r, n, l.lanes, p.C);   // (before the wait for the statistics)
+        if (res) q.load(res + c0, r, n, l.lanes, p.C);
+        if (k.s != s || k.pass != pass) {
+            sync_workers();
+            if (!k.template load<false>(p, l, s, pass, true)) return false;
+        }
+        if (owner) k.put_stats(p, l);
+        for (; r < n; r += U * l.lanes) {
+            uint32_t words[U][P];
+            if (drop) {
+#pragma unroll
+                for (int u = 0; u < U; ++u) rng.words<VN>((uint64_t)(from + (r + u * l.lanes) * p.C + c0), words[u]);
+            }
+#pragma unroll
+            for (int h = 0; h < Constants<VN>::QUADS; ++h) {
+                float2 a[PAIRS], b[PAIRS];
+                k.read(l, K_A, h, a), k.read(l, K_B, h, b);
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+#pragma unroll
+                    for (int i = 0; i < PAIRS; ++i) {
+                        const int j = h * PAIRS + i;
+                        float2 z = fma2(pair_of(v.v[u], j), a[i], b[i]);
+                        if (res) z = add2(z, pair_of(q.v[u], j));
+                        z = act2(act, z);
+                        if (drop) z = drop2<VN>(p, words[u], j, z);
+                        set_pair(v.v[u], j, z);
+                    }
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (r + u * l.lanes < n) v.v[u].store(y + (r + u * l.lanes) * p.C + c0);
+            v.load(x + c0, r + U * l.lanes, n, l.lanes, p.C);
+            if (res) q.load(res + c0, r + U * l.lanes, n, l.lanes, p.C);
+        }
+    }
+    return true;
+}
+
+// ------------------------------------------------------------ backward ----
+// Rows of what both passes of the backward read, and gz of a pair of them.
+template <typename T, int VN, int ACT, int DROP, int U>
+struct BackwardRows {
+    static constexpr int P = (VN + 1) / 2;
+    Rows<T, VN, U> x, g, res;
+    uint32_t words[U][P];
+    // `from`: the element that the lumps' first one is
+    __device__ __forceinline__ void load(const NormAct &p, const Columns &l, int64_t from, int r, int n) {
+        x.load(static_cast<const T *>(p.x) + from, r, n, l.lanes, p.C);
+        g.load(static_cast<const T *>(p.g) + from, r, n, l.lanes, p.C);
+        if (p.residual) res.load(static_cast<const T *>(p.residual) + from, r, n, l.lanes, p.C);
+    }
+    __device__ __forceinline__ void draw(const NormAct &p, const Columns &l, const Philox<DROP != 1> &rng, int64_t from, int r) {
+        if (DROP < 0 ? p.drop.on : DROP) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) rng.words<VN>((uint64_t)(from + (r + u * l.lanes) * p.C), words[u]);
+        }
+    }
+    __device__ __forceinline__ float2 gz(const NormAct &p, int u, int j, float2 xc, float2 a, float2 b) const {
+        float2 z = fma2(xc, a, b);
+        if (p.residual) z = add2(z, pair_of(res.v[u], j));
+        const float2 v = act2_backward(ACT < 0 ? p.act : ACT, z, pair_of(g.v[u], j));
+        return (DROP < 0 ? p.drop.on : DROP) ? drop2<VN>(p, words[u], j, v) : v;
+    }
+};
+template <typename T, int VN>
+constexpr int BACKWARD_ROWS = sizeof(T) == 4 && VN == 8 ? 1 : 2;
+
+template <typename T, int VN, int ACT, int DROP>
+__device__ __forceinline__ void bwd_sums_piece(const NormAct &p, const Columns &l, const Philox<DROP != 1> &rng, Constants<VN> &k, int64_t piece, int64_t s, int64_t lo, int n,
+                                               float2 *fold) {
+    constexpr int U = BACKWARD_ROWS<T, VN>, P = (VN + 1) / 2, PAIRS = Constants<VN>::PAIRS;
+    for (int pass = 0; pass < l.passes; ++pass) {
+        const int lump = pass * l.cols + l.col;
+        const int64_t from = lo * p.C + lump * VN;
+        float2 a[P], b[P];
+#pragma unroll
+        for (int j = 0; j < P; ++j) a[j] = b[j] = both(0.f);
+        int r = lump < l.lumps && l.lane < l.lanes ? l.lane : n;
+        BackwardRows<T, VN, ACT, DROP, U> in;
+        in.load(p, l, from, r, n);
+        if (k.s != s || k.pass != pass) {
+            sync_workers();
+            k.template load<true>(p, l, s, pass, false);
+        }
+        for (; r < n; r += U * l.lanes) {
+            in.draw(p, l, rng, from, r);
+#pragma unroll
+            for (int h = 0; h < Constants<VN>::QUADS; ++h) {
+                float2 mu[PAIRS], fa[PAIRS], fb[PAIRS];
+                k.read(l, K_MU, h, mu), k.read(l, K_A, h, fa), k.read(l, K_B, h, fb);
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    if (r + u * l.lanes < n)
+#pragma unroll
+                        for (int i = 0; i < PAIRS; ++i) {
+                            const int j = h * PAIRS + i;
+                            const float2 xc = add2(pair_of(in.x.v[u], j), mu[i]), gz = in.gz(p, u, j, xc, fa[i], fb[i]);
+                            a[j] = add2(a[j], gz), b[j] = fma2(gz, xc, b[j]);
+                        }
+            }
+            in.load(p, l, from, r + U * l.lanes, n);
+        }
+        fold_lanes<VN>(l, pass, a, b, fold, [&](int c, float sa, float sb) {
+            p.rec[piece * p.C + c] = make_float2(sa, sb * __ldg(p.rstd + s * p.G + group_of(p, c)));
+        });
+    }
+}
+
+template <typename T, int VN, int ACT, int DROP>
+__device__ __forceinline__ bool bwd_apply_piece(const NormAct &p, const Columns &l, const Philox<DROP != 1> &rng, Constants<VN> &k, int64_t s, int64_t lo, int n) {
+    constexpr int U = BACKWARD_ROWS<T, VN>, PAIRS = Constants<VN>::PAIRS;
+    T *dx = static_cast<T *>(p.dx), *dres = static_cast<T *>(p.dresidual);
+    for (int pass = 0; pass < l.passes; ++pass) {
+        const int lump = pass * l.cols + l.col;
+        const int64_t from = lo * p.C + lump * VN;
+        int r = lump < l.lumps && l.lane < l.lanes ? l.lane : n;
+        BackwardRows<T, VN, ACT, DROP, U> in;
+        in.load(p, l, from, r, n);   // (before the wait for the sums)
+        if (k.s != s || k.pass != pass) {
+            sync_workers();
+            if (!k.template load<true>(p, l, s, pass, true)) return false;
+        }
+        for (; r < n; r += U * l.lanes) {
+            in.draw(p, l, rng, from, r);
+#pragma unroll
+            for (int h = 0; h < Constants<VN>::QUADS; ++h) {
+                float2 mu[PAIRS], fa[PAIRS], fb[PAIRS], m1[PAIRS], m2[PAIRS];
+                k.read(l, K_MU, h, mu), k.read(l, K_A, h, fa), k.read(l, K_B, h, fb), k.read(l, K_M1, h, m1), k.read(l, K_M2, h, m2);
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+#pragma unroll
+                    for (int i = 0; i < PAIRS; ++i) {
+                        const int j = h * PAIRS + i;
+                        const float2 xc = add2(pair_of(in.x.v[u], j), mu[i]), gz = in.gz(p, u, j, xc, fa[i], fb[i]);
+                        set_pair(in.g.v[u], j, gz);
+                        set_pair(in.x.v[u], j, fma2(gz, fa[i], fma2(xc, m2[i], m1[i])));
+                    }
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (r + u * l.lanes < n) {
+                    const int64_t at = from + (r + u * l.lanes) * p.C;
+                    if (dres) in.g.v[u].store(dres + at);
+                    in.x.v[u].store(dx + at);
+                }
+            in.load(p, l, from, r + U * l.lanes, n);
+        }
+    }
+    return true;
+}
+
+// ------------------------------------------------------------ merging ----
+// Who merges: the block's workers, or one warp.
+struct BlockTeam {
+    static constexpr int SIZE = NA_THREADS;
+    __device__ __forceinline__ static int rank() { return threadIdx.x; }
+    __device__ __forceinline__ static void sync() { sync_workers(); }
+};
+struct WarpTeam {
+    static constexpr int SIZE = 32;
+    __device__ __forceinline__ static int rank() { return threadIdx.x & 31; }
+    __device__ __forceinline__ static void sync() { __syncwarp(); }
+};
+
+// Merges the pieces of a window: a part of what merge_groups does, where records are many.
+template <bool BACKWARD, typename Team>
+__device__ __forceinline__ void merge_window(const NormAct &p, const Records &r, float2 *to) {
+    for (int g = Team::rank(); g < p.G; g += Team::SIZE) {
+        RecordSums<BACKWARD> sums;
+        sums.add(r, p.G, g, 0, 1);
+        to[g] = sums.done(r, p.G, g, (float)p.W);
+    }
+}
+
+// Lanes of a warp that share a group's channels.
+template <typename Team>
+__device__ __forceinline__ int lanes_of_group(const NormAct &p) {
+    int share = 32;
+    while (share > 1 && (Team::SIZE / share < p.G || share / 2 >= p.W)) share /= 2;
+    return share;
+}
+
+// The records of a piece's groups, of `n` rows, from its channels' (`channel(c)`, visible to the team).
+template <bool BACKWARD, typename Team, typename Channel>
+__device__ __forceinline__ void group_records(const NormAct &p, int share, float inverse, int64_t piece, float n, Channel channel) {
+    const int l = Team::rank() % share;
+    const auto sum = [&](float v) {
+        for (int o = share / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        return v;
+    };
+    for (int g0 = 0; g0 < p.G; g0 += Team::SIZE / share) {   // (the same rounds for all lanes of a warp)
+        const int g = g0 + Team::rank() / share, c0 = min(g, p.G - 1) * p.W, end = g < p.G ? p.W : 0;
+        float a = 0.f, b = 0.f;
+        if constexpr (BACKWARD) {
+#pragma unroll 4
+            for (int i = l; i < end; i += share) {
+                const float2 v = channel(c0 + i);
+                const float w = p.weight ? __ldg(p.weight + c0 + i) : 1.f;
+                a += w * v.x, b += w * v.y;
+            }
+            a = sum(a), b = sum(b);
+        } else {   // the mean first, then squares about it
+            const float k = channel(c0).x;
+#pragma unroll 4
+            for (int i = l; i < end; i += share) a += channel(c0 + i).x - k;
+            a = k + sum(a) * inverse;
+#pragma unroll 4
+            for (int i = l; i < end; i += share) {
+                const float2 v = channel(c0 + i);
+                b += v.y + n * (v.x - a) * (v.x - a);
+            }
+            b = sum(b);
+        }
+        if (g < p.G && l == 0) p.of_piece[piece * p.G + g] = make_float2(a, b);
+    }
+}
+
+// Counts what the team has written; true in all of its threads where that was the last of `of`, and then the others' is there to be read.
+template <typename Team>
+__device__ __forceinline__ bool brings_the_last(int *count, int of, int *told) {
+    Team::sync();
+    if (Team::rank() == 0) {
+        __threadfence();
+        *told = atomicAdd(count, 1);
+    }
+    Team::sync();
+    const bool last = *told == of - 1;
+    Team::sync();   // (before it is told again)
+    if (last) __threadfence();
+    return last;
+}
+
+// After the team has written the records of piece (chunk, s).
+template <bool BACKWARD, typename Team>
+__device__ __forceinline__ void count_piece(const NormAct &p, const Span &v, int chunk, int64_t s, int *told) {
+    if (p.window > 1) {
+        const int w = (chunk - v.b0) / p.window, b = v.b0 + w * p.window, pieces = min(p.window, v.b1 - b + 1);
+        const int64_t number = first_window(p, v, s) + w, from = (int64_t)b * p.rows;
+        if (!brings_the_last<Team>(window_count(p) + number, pieces, told)) return;
+        const int64_t lo = max(p.offsets[s], from), hi = min(p.offsets[s + 1], from + (int64_t)pieces * p.rows);
+        merge_window<BACKWARD, Team>(p, records_of(p.of_piece + (b + s) * p.G, pieces, lo, hi, from, p.rows), p.of_window + number * p.G);
+    }
+    Team::sync();
+    if (Team::rank() == 0) {
+        __threadfence();
+        atomicAdd(sample_count(p) + s, 1);
+        if (BACKWARD && p.dweight) atomicAdd(p.control + WINDOWS_DONE, 1);
+    }
+}
+
+// dweight and dbias of some channels: the pieces' sums in a fixed order, in fp64 at last.
+__device__ __noinline__ void affine_gradients(const NormAct &p, int tile, double2 *scratch) {
+    constexpr int DEEP = NA_THREADS / AFFINE_CHANNELS;
+    const int lane = threadIdx.x % AFFINE_CHANNELS, q = threadIdx.x / AFFINE_CHANNELS, c = tile * AFFINE_CHANNELS + lane;
+    const int64_t pieces = p.N / p.rows + p.S;   // (numbers that no piece has hold zeros)
+    float a = 0.f, b = 0.f;
+    if (c < p.C)
+#pragma unroll 8
+        for (int64_t i = q; i < pieces; i += DEEP) {
+            const float2 v = __ldcg(p.rec + i * p.C + c);
+            a += v.x, b += v.y;
+        }
+    sync_workers();
+    scratch[threadIdx.x] = make_double2(a, b);
+    sync_workers();
+    if (q == 0 && c < p.C) {
+        double da = 0.0, db = 0.0;
+        for (int i = 0; i < DEEP; ++i) da += scratch[i * AFFINE_CHANNELS + lane].x, db += scratch[i * AFFINE_CHANNELS + lane].y;
+        p.dbias[c] = (float)da, p.dweight[c] = (float)db;
+    }
+}
+
+// ------------------------------------------------------------ the kernel ----
+template <int VN, bool BACKWARD>
+size_t shared_bytes(int C) {
+    const Columns l(C, VN, 0);
+    return (size_t)std::max(VN, 2) * NA_THREADS * sizeof(float2) + (size_t)(BACKWARD ? 8 : 3) * l.cols * VN * sizeof(float) +
+           (size_t)(2 * NA_THREADS + l.cols * VN + 2) * sizeof(float2);
+}
+
+// ACT, DROP = -1: as the arguments say; DROP = 0: none, 1: the seed is in the arguments, 2: on the device.
+template <typename T, int VN, int ACT, int DROP, bool BACKWARD>
+__global__ void __launch_bounds__(NA_THREADS, BACKWARD ? 3 : 4) na_kernel(const __grid_constant__ NormAct p) {
+    start_after_previous();
+    extern __shared__ __align__(128) char shared[];
+    __shared__ int next, told;
+    float2 *fold = reinterpret_cast<float2 *>(shared);   // sums of threads, or records that are merged
+    const Columns l(p.C, VN, threadIdx.x);
+    Constants<VN> k_sums, k_apply;
+    k_apply.at = reinterpret_cast<float *>(fold + (VN < 2 ? 2 : VN) * NA_THREADS);
+    k_sums.at = k_apply.at + 5 * l.cols * VN;
+    k_apply.scratch = reinterpret_cast<float4 *>(k_apply.at + ((BACKWARD ? 8 : 3) * l.cols * VN + 3) / 4 * 4), k_apply.stats = reinterpret_cast<float2 *>(k_apply.scratch + NA_THREADS);
+    const Philox<DROP != 1> rng(p.drop);
+    const int tiles = BACKWARD && p.dweight ? (p.C + AFFINE_CHANNELS - 1) / AFFINE_CHANNELS : 0;
+    for (;;) {
+        __syncthreads();
+        if (threadIdx.x == 0) next = atomicAdd(p.control + TICKET, 1);
+        __syncthreads();
+        const int ticket = next;
+        if (ticket >= 2 * p.chunks + tiles) return;
+        if (BACKWARD && ticket >= 2 * p.chunks) {
+            if (!wait_for(p.control + WINDOWS_DONE, p.control[WINDOWS], p.status)) return;
+            affine_gradients(p, ticket - 2 * p.chunks, reinterpret_cast<double2 *>(fold));
+            continue;
+        }
+        int chunk;
+        const bool sums = take_ticket(p, ticket, &chunk);
+        const int64_t row0 = (int64_t)chunk * p.rows, row1 = min(p.N, row0 + p.rows);
+        for (int64_t s = last_not_over(p.S, row0, [&](int64_t q) { return p.offsets[q]; }); s < p.S && p.offsets[s] < row1; ++s) {
+            const int64_t lo = max(row0, p.offsets[s]), hi = min(row1, p.offsets[s + 1]);
+            if (hi <= lo) continue;   // a sample without rows
+            if (sums) {
+                if constexpr (BACKWARD) bwd_sums_piece<T, VN, ACT, DROP>(p, l, rng, k_sums, chunk + s, s, lo, (int)(hi - lo), fold);
+                else stats_piece<T, VN>(p, l, chunk + s, lo, (int)(hi - lo), fold);
+                sync_workers();
+                const float2 *channels = p.rec + (chunk + s) * p.C;   // (what this block has written)
+                group_records<BACKWARD, BlockTeam>(p, lanes_of_group<BlockTeam>(p), 1.f / (float)p.W, chunk + s, (float)(hi - lo), [&](int c) { return __ldcg(channels + c); });
+                count_piece<BACKWARD, BlockTeam>(p, p.spans[s], chunk, s, &told);
+            } else {
+                bool there;
+                if constexpr (BACKWARD) there = bwd_apply_piece<T, VN, ACT, DROP>(p, l, rng, k_apply, s, lo, (int)(hi - lo));
+                else there = apply_piece<T, VN, ACT, DROP>(p, l, rng, k_apply, s, lo, (int)(hi - lo), chunk == p.spans[s].b0);
+                if (!there) return;
+            }
+        }
+    }
+}
+
+// ------------------------------------------------------------ the ring ----
+// The same tickets where rows are whole lumps of eight channels at 16-byte addresses, up to 1024 channels.  A warp, the producer, takes
+// the tickets and brings their rows, which lie side by side, by bulk copies into a ring of tiles in shared memory; eight warps work on
+// them; the sums of a piece go to another warp, the clerk, which folds them, writes the record, counts it and merges.  So whatever a
+// ticket waits for (its number, the samples' offsets, the first bytes) passes while tiles before it are worked on, and rows are not
+// kept waiting by records: with both done by the workers, between tickets, a ticket of 64 KB took 4.7 us and 2 more to be counted.
+enum { TILE_SUMS = 0, TILE_APPLY = 1, TILE_AFFINE = 2, TILE_END = 3, TILE_NONE = 4 };
+constexpr int RING_CHANNELS = 1024;                // at most (their constants take room from the ring)
+constexpr int RING_STAGES = 8;                     // at most
+constexpr int FOLD_SLOTS = 2;                      // pieces on their way to the clerk
+constexpr int FOLD_STRIDE = NA_THREADS + 2;        // of a channel of the lumps (two more: without bank conflicts)
+constexpr int RING_THREADS = NA_THREADS + 64;
+constexpr int RING_BLOCKS = 2;                     // on a multiprocessor
+struct __align__(16) Tile {
+    int kind, s, chunk, n;       // n rows
+    int64_t from;                // the first element
+    int last;                    // sums: the last of a piece; apply: the first of a sample
+};
+struct Piece { int kind, s, chunk, rows; };
+
+struct Ring {
+    uint64_t full[RING_STAGES], empty[RING_STAGES], folded[FOLD_SLOTS], taken[FOLD_SLOTS];
+    Tile tiles[RING_STAGES];
+    Piece pieces[FOLD_SLOTS];
+    int told, abort;
+};
+// (behind the ring's tiles) two slots of sums, the channels' values in the piece's first row for each, constants
+struct RingMemory {
+    char *stages;
+    float2 *fold;
+    float *firsts, *constants;
+    float2 *stats, *scratch;
+    __device__ __forceinline__ RingMemory(const NormAct &p, char *shared) {
+        stages = shared;
+        fold = reinterpret_cast<float2 *>(shared + (size_t)p.stages * p.stage_bytes);
+        scratch = fold + FOLD_SLOTS * 8 * FOLD_STRIDE;
+        stats = scratch + 2 * NA_THREADS;   // (scratch: 256 sums of two doubles at most)
+        constants = reinterpret_cast<float *>(stats + p.C);
+        firsts = constants + 3 * p.C;   // (forward alone)
+    }
+};
+inline size_t ring_bytes(int C, bool backward) {   // without the tiles
+    return (size_t)(FOLD_SLOTS * 8 * FOLD_STRIDE + 2 * NA_THREADS + C) * sizeof(float2) + (size_t)(backward ? 8 : 3 + FOLD_SLOTS) * C * sizeof(float);
+}
+
+__device__ __forceinline__ void bulk_copy(uint32_t to, const void *from, uint32_t bytes, uint32_t bar, uint64_t policy) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1], %2, [%3], %4;" ::"r"(to), "l"(from), "r"(bytes), "r"(bar), "l"(policy)
+                 : "memory");
+}
+__device__ __forceinline__ void expect_bytes(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+// A place in a ring of `size`, and the parity of its round.
+struct Place {
+    int at = -1, parity = 0;
+    __device__ __forceinline__ void next(int size) {
+        if (++at == size) at = 0, parity ^= 1;
+    }
+};
+
+template <typename T, bool BACKWARD>
+__device__ __forceinline__ void ring_producer(const NormAct &p, Ring &ring, const RingMemory &m) {
+    const int lane = threadIdx.x & 31, tiles = BACKWARD && p.dweight ? (p.C + AFFINE_CHANNELS - 1) / AFFINE_CHANNELS : 0;
+    const uint32_t step = (uint32_t)p.tile_rows * p.C * sizeof(T), stages = tc::smem_u32(m.stages);
+    uint64_t keep, drop;
+    asm volatile("createpolicy.fractional.L2::evict_last.b64 %0, 1.0;" : "=l"(keep));
+    asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(drop));
+    Place place;
+    int brought = 0;
+    const auto push = [&](const Tile &t) -> bool {
+        place.next(p.stages);
+        if (brought >= p.stages &&
+            !__all_sync(0xffffffffu, tc::mbar_wait_abortable(tc::smem_u32(&ring.empty[place.at]), place.parity ^ 1, NA_STATUS, p.status, &ring.abort))) {
+            return false;
+        }
+        if (lane == 0) {
+            ring.tiles[place.at] = t;
+            const uint32_t bar = tc::smem_u32(&ring.full[place.at]);
+            if (t.kind <= TILE_APPLY) {
+                const uint32_t each = (uint32_t)t.n * p.C * sizeof(T);
+                const bool stats = !BACKWARD && t.kind == TILE_SUMS;   // (of x alone)
+                uint32_t to = stages + (uint32_t)place.at * p.stage_bytes;
+                const uint64_t policy = t.kind == TILE_SUMS ? keep : drop;
+                expect_bytes(bar, each * ((BACKWARD ? 2 : 1) + (p.residual && !stats)));
+                bulk_copy(to, static_cast<const T *>(p.x) + t.from, each, bar, policy), to += step;
+                if (BACKWARD) bulk_copy(to, static_cast<const T *>(p.g) + t.from, each, bar, policy), to += step;
+                if (p.residual && !stats) bulk_copy(to, static_cast<const T *>(p.residual) + t.from, each, bar, policy);
+            } else {
+                tc::mbar_arrive(bar);
+            }
+        }
+        ++brought;
+        return true;
+    };
+    const auto all = [&]() -> bool {
+        int ticket = 0, upcoming = 0;
+        if (lane == 0) ticket = atomicAdd(p.control + TICKET, 1);
+        ticket = __shfl_sync(0xffffffffu, ticket, 0);
+        for (;; ticket = __shfl_sync(0xffffffffu, upcoming, 0)) {
+            if (ticket >= 2 * p.chunks + tiles) return push(Tile{TILE_END, 0, 0, 0, 0, 0});
+            if (lane == 0) upcoming = atomicAdd(p.control + TICKET, 1);
+            if (ticket >= 2 * p.chunks) {
+                if (!push(Tile{TILE_AFFINE, 0, ticket - 2 * p.chunks, 0, 0, 0})) return false;
+                continue;
+            }
+            int chunk;
+            const bool sums = take_ticket(p, ticket, &chunk);
+            const int tile_rows = sums ? p.sums_tile_rows : p.tile_rows;
+            const int64_t row0 = (int64_t)chunk * p.rows, row1 = min(p.N, row0 + p.rows);
+            for (int64_t s = last_not_over(p.S, row0, [&](int64_t q) { return p.offsets[q]; }); s < p.S; ++s) {
+                const int64_t at = p.offsets[s], lo = max(row0, at), hi = min(row1, p.offsets[s + 1]);
+                if (at >= row1) break;
+                const bool owner = !BACKWARD && !sums && chunk == p.spans[s].b0;   // (of the statistics)
+                for (int64_t r = lo; r < hi; r += tile_rows) {
+                    const int n = (int)min((int64_t)tile_rows, hi - r);
+                    if (!push(Tile{sums ? TILE_SUMS : TILE_APPLY, (int)s, chunk, n, r * p.C, sums ? r + n == hi : owner && r == lo})) return false;
+                }
+            }
+        }
+    };
+    if (!all()) {   // shared memory is not given back under copies in flight
+        const int behind = min(brought, p.stages);
+        Place q;
+        for (int j = 0; j < brought; ++j) {
+            q.next(p.stages);
+            if (j >= brought - behind) tc::mbar_wait(tc::smem_u32(&ring.full[q.at]), q.parity, NA_STATUS, p.status);
+        }
+    }
+}
+
+// Whether whole rows of columns make a warp (64 channels: 8 columns, 4 rows): its lanes are then folded before the clerk has them.
+__device__ __forceinline__ bool warps_fold(const Columns &l) { return l.cols < 32 && 32 % l.cols == 0; }
+
+// Folds the sums of pieces over the row lanes and takes them from there.
+template <bool BACKWARD>
+__device__ __forceinline__ void ring_clerk(const NormAct &p, Ring &ring, const RingMemory &m) {
+    const int lane = threadIdx.x & 31;
+    const Columns l(p.C, 8, 0);
+    const int lanes = warps_fold(l) ? NA_THREADS / 32 : l.lanes, share = lanes_of_group<WarpTeam>(p);
+    const float inverse = 1.f / (float)p.W;
+    Place slot;
+    for (;;) {
+        slot.next(FOLD_SLOTS);
+        if (!__all_sync(0xffffffffu, tc::mbar_wait_abortable(tc::smem_u32(&ring.folded[slot.at]), slot.parity, NA_STATUS, p.status, &ring.abort))) return;
+        const Piece piece = ring.pieces[slot.at];
+        if (piece.kind == TILE_END) return;
+        float2 *fold = m.fold + slot.at * 8 * FOLD_STRIDE;
+        const float *firsts = m.firsts + slot.at * p.C;
+        const int64_t number = piece.chunk + (int64_t)piece.s;
+        const float each = 1.f / (float)piece.rows;
+        for (int c = lane; c < p.C; c += 32) {
+            float2 *from = fold + c % 8 * FOLD_STRIDE + c / 8;
+            float a = 0.f, b = 0.f;
+#pragma unroll 8
+            for (int q = 0; q < lanes; ++q) {
+                const float2 v = from[q * l.cols];
+                a += v.x, b += v.y;
+            }
+            if constexpr (BACKWARD) {
+                b *= __ldg(p.rstd + (int64_t)piece.s * p.G + group_of(p, c));
+                if (p.dweight) p.rec[number * p.C + c] = make_float2(a, b);
+            } else {
+                const float off = a * each;
+                b = fmaxf(b - a * off, 0.f), a = firsts[c] + off;
+            }
+            *from = make_float2(a, b);
+        }
+        __syncwarp();
+        group_records<BACKWARD, WarpTeam>(p, share, inverse, number, (float)piece.rows, [&](int c) { return fold[c % 8 * FOLD_STRIDE + c / 8]; });
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(tc::smem_u32(&ring.taken[slot.at]));
+        count_piece<BACKWARD, WarpTeam>(p, p.spans[piece.s], piece.chunk, piece.s, &ring.told);
+    }
+}
+
+// The workers' warps wait for tiles each by itself, and meet where the sample changes.  One whose wait has run out comes to the next
+// meeting with that, whichever it is, and then all of them leave: a meeting is the first barrier that a warp comes to after any tile.
+template <typename T, int ACT, int DROP, bool BACKWARD>
+__device__ __forceinline__ void ring_worker(const NormAct &p, Ring &ring, const RingMemory &m) {
+    constexpr int VN = 8, P = 4, UNROLL = BACKWARD && DROP ? 1 : 2;   // (more spills registers)
+    const Columns l(p.C, VN, threadIdx.x);
+    const Philox<DROP != 1> rng(p.drop);
+    const bool mine = l.lane < l.lanes;
+    const int c0 = l.col * VN, step = l.lanes * p.C;   // elements from one of a thread's rows to its next
+    const int tensor = p.tile_rows * p.C;              // elements from one tensor's tile to the next one's
+    Constants<8> k_sums, k_apply;
+    k_apply.at = m.constants, k_sums.at = m.constants + 5 * p.C;
+    k_apply.stats = m.stats, k_apply.scratch = reinterpret_cast<float4 *>(m.scratch);
+    Place place, slot;
+    int pieces = 0;
+    Tile t;
+    const auto next_tile = [&] {
+        place.next(p.stages);
+        if (__all_sync(0xffffffffu, tc::mbar_wait(tc::smem_u32(&ring.full[place.at]), place.parity, NA_STATUS, p.status))) t = ring.tiles[place.at];
+        else t.kind = TILE_NONE;
+    };
+    const auto release = [&] {
+        __syncwarp();
+        if ((threadIdx.x & 31) == 0) tc::mbar_arrive(tc::smem_u32(&ring.empty[place.at]));
+    };
+    const auto rows_at = [&] { return reinterpret_cast<const T *>(m.stages + (size_t)place.at * p.stage_bytes) + c0; };
+    // A slot for sums; false: the clerk has not come for the ones before.
+    const auto next_slot = [&]() -> bool {
+        slot.next(FOLD_SLOTS);
+        return ++pieces <= FOLD_SLOTS || __all_sync(0xffffffffu, tc::mbar_wait(tc::smem_u32(&ring.taken[slot.at]), slot.parity ^ 1, NA_STATUS, p.status));
+    };
+    const auto send = [&](const Piece &piece) {
+        if (threadIdx.x == 0) ring.pieces[slot.at] = piece;
+        __syncwarp();
+        if ((threadIdx.x & 31) == 0) tc::mbar_arrive(tc::smem_u32(&ring.folded[slot.at]));
+    };
+    next_tile();
+    for (;;) {
+        if (t.kind == TILE_SUMS) {
+            float2 a[P], b[P], k[P], fa[P], fb[P];   // k: what is taken off x
+            const int s = t.s, chunk = t.chunk;
+            int rows = 0;
+            if (BACKWARD && k_sums.s != s) {
+                if (!sync_workers_and(true)) break;
+                k_sums.load<true>(p, l, s, 0, false);
+            }
+            const bool free = next_slot();
+#pragma unroll
+            for (int j = 0; j < P; ++j) a[j] = b[j] = both(0.f);
+            if constexpr (BACKWARD) {
+                k_sums.read_all(l, K_MU, k), k_sums.read_all(l, K_A, fa), k_sums.read_all(l, K_B, fb);
+            } else {
+                Lump<T, VN> v;
+                v.load(rows_at());
+#pragma unroll
+                for (int j = 0; j < P; ++j) k[j] = neg2(pair_of(v, j));
+                if (l.lane == 0 && free) {
+#pragma unroll
+                    for (int q = 0; q < VN; ++q) m.firsts[slot.at * p.C + c0 + q] = v.get(q);
+                }
+            }
+            for (bool more = true; more;) {
+                const T *x = rows_at();
+                if (mine)
+#pragma unroll UNROLL
+                    for (int r = l.lane, at = l.lane * p.C; r < t.n; r += l.lanes, at += step) {
+                        BackwardRows<T, VN, ACT, DROP, 1> in;
+                        in.x.v[0].load(x + at);
+                        if constexpr (BACKWARD) {
+                            in.g.v[0].load(x + tensor + at);
+                            if (p.residual) in.res.v[0].load(x + 2 * tensor + at);
+                            if (DROP) rng.words<VN>((uint64_t)(t.from + at + c0), in.words[0]);
+                        }
+#pragma unroll
+                        for (int j = 0; j < P; ++j) {
+                            const float2 xc = add2(pair_of(in.x.v[0], j), k[j]);
+                            if constexpr (BACKWARD) {
+                                const float2 gz = in.gz(p, 0, j, xc, fa[j], fb[j]);
+                                a[j] = add2(a[j], gz), b[j] = fma2(gz, xc, b[j]);
+                            } else {
+                                a[j] = add2(a[j], xc), b[j] = fma2(xc, xc, b[j]);
+                            }
+                        }
+                    }
+                rows += t.n;
+                more = !t.last;
+                release();
+                next_tile();
+                if (t.kind == TILE_NONE) more = false;
+            }
+            if (!free) t.kind = TILE_NONE;
+            if (t.kind != TILE_NONE) {
+                if (warps_fold(l)) {   // over the warp's row lanes first
+                    for (int o = 16; o >= l.cols; o >>= 1)
+#pragma unroll
+                        for (int j = 0; j < P; ++j) {
+                            a[j] = add2(a[j], make_float2(__shfl_xor_sync(0xffffffffu, a[j].x, o), __shfl_xor_sync(0xffffffffu, a[j].y, o)));
+                            b[j] = add2(b[j], make_float2(__shfl_xor_sync(0xffffffffu, b[j].x, o), __shfl_xor_sync(0xffffffffu, b[j].y, o)));
+                        }
+                }
+                if (!warps_fold(l) || (threadIdx.x & 31) < l.cols) {
+                    float2 *fold = m.fold + slot.at * 8 * FOLD_STRIDE + (warps_fold(l) ? (threadIdx.x >> 5) * l.cols + (threadIdx.x & 31) : threadIdx.x);
+#pragma unroll
+                    for (int i = 0; i < VN; ++i) fold[i * FOLD_STRIDE] = i % 2 ? make_float2(a[i / 2].y, b[i / 2].y) : make_float2(a[i / 2].x, b[i / 2].x);
+                }
+                send(Piece{TILE_SUMS, s, chunk, rows});
+            }
+        } else if (t.kind == TILE_APPLY) {
+            const int s = t.s;
+            if (k_apply.s != s) {
+                if (!sync_workers_and(true)) break;
+                if (!k_apply.load<BACKWARD>(p, l, s, 0, true)) break;
+            }
+            float2 mu[P], fa[P], fb[P], m1[P], m2[P];
+            k_apply.read_all(l, K_A, fa), k_apply.read_all(l, K_B, fb);
+            if constexpr (BACKWARD) k_apply.read_all(l, K_MU, mu), k_apply.read_all(l, K_M1, m1), k_apply.read_all(l, K_M2, m2);
+            do {
+                const T *x = rows_at();
+                if (!BACKWARD && t.last) k_apply.put_stats(p, l);
+                if (mine)
+#pragma unroll UNROLL
+                    for (int r = l.lane, at = l.lane * p.C; r < t.n; r += l.lanes, at += step) {
+                        const int64_t to = t.from + at + c0;
+                        BackwardRows<T, VN, ACT, DROP, 1> in;
+                        in.x.v[0].load(x + at);
+                        if constexpr (BACKWARD) in.g.v[0].load(x + tensor + at);
+                        if (p.residual) in.res.v[0].load(x + (BACKWARD ? 2 : 1) * tensor + at);
+                        if (DROP) rng.words<VN>((uint64_t)to, in.words[0]);
+#pragma unroll
+                        for (int j = 0; j < P; ++j) {
+                            if constexpr (BACKWARD) {
+                                const float2 xc = add2(pair_of(in.x.v[0], j), mu[j]), gz = in.gz(p, 0, j, xc, fa[j], fb[j]);
+                                set_pair(in.g.v[0], j, gz);
+                                set_pair(in.x.v[0], j, fma2(gz, fa[j], fma2(xc, m2[j], m1[j])));
+                            } else {
+                                float2 z = fma2(pair_of(in.x.v[0], j), fa[j], fb[j]);
+                                if (p.residual) z = add2(z, pair_of(in.res.v[0], j));
+                                z = act2(ACT, z);
+                                if (DROP) z = drop2<VN>(p, in.words[0], j, z);
+                                set_pair(in.x.v[0], j, z);
+                            }
+                        }
+                        if (BACKWARD && p.dresidual) in.g.v[0].store_streaming(static_cast<T *>(p.dresidual) + to);
+                        in.x.v[0].store_streaming(static_cast<T *>(BACKWARD ? p.dx : p.y) + to);
+                    }
+                release();
+                next_tile();
+            } while (t.kind == TILE_APPLY && t.s == s);
+        } else {
+            if (!sync_workers_and(t.kind != TILE_NONE)) break;
+            if (t.kind == TILE_END) {
+                if (!next_slot()) break;
+                send(Piece{TILE_END, 0, 0, 0});
+                return;
+            }
+            if (!wait_for(p.control + WINDOWS_DONE, p.control[WINDOWS], p.status)) break;
+            affine_gradients(p, t.chunk, reinterpret_cast<double2 *>(m.scratch));
+            release();
+            next_tile();
+        }
+    }
+    ring.abort = 1;
+}
+
+template <typename T, int ACT, int DROP, bool BACKWARD>
+__global__ void __launch_bounds__(RING_THREADS, RING_BLOCKS) na_ring_kernel(const __grid_constant__ NormAct p) {
+    extern __shared__ __align__(128) char shared[];
+    __shared__ Ring ring;
+    if (threadIdx.x == 0) {
+        for (int q = 0; q < p.stages; ++q) tc::mbar_init(tc::smem_u32(&ring.full[q]), 1), tc::mbar_init(tc::smem_u32(&ring.empty[q]), NA_THREADS / 32);
+        for (int q = 0; q < FOLD_SLOTS; ++q) tc::mbar_init(tc::smem_u32(&ring.folded[q]), NA_THREADS / 32), tc::mbar_init(tc::smem_u32(&ring.taken[q]), 1);
+        ring.abort = 0;
+        tc::fence_mbar_init();
+    }
+    start_after_previous();
+    __syncthreads();
+    const RingMemory m(p, shared);
+    if (threadIdx.x < NA_THREADS) ring_worker<T, ACT, DROP, BACKWARD>(p, ring, m);
+    else if (threadIdx.x < NA_THREADS + 32) ring_producer<T, BACKWARD>(p, ring, m);
+    else ring_clerk<BACKWARD>(p, ring, m);
+}
+
+template <typename T, int ACT, int DROP, bool BACKWARD>
+int run_ring(const NormAct &p, cudaStream_t stream) {
+    const auto kernel = na_ring_kernel<T, ACT, DROP, BACKWARD>;
+    static std::atomic<uint64_t> allowed;
+    if (int rc = allow_shared_memory((const void *)kernel, &allowed, true)) return rc;
+    const int64_t tickets = 2 * (int64_t)p.chunks;
+    launch_after(kernel, (unsigned)std::min<int64_t>(tickets, RING_BLOCKS * num_sms()), RING_THREADS, (size_t)p.stages * p.stage_bytes + ring_bytes(p.C, BACKWARD), stream, p);
+    PCX_LAUNCH_CHECK();
+    return PCX_OK;
+}
+
+template <typename T, int VN, int ACT, int DROP, bool BACKWARD>
+int run_kernel(const NormAct &p, cudaStream_t stream) {
+    const auto kernel = na_kernel<T, VN, ACT, DROP, BACKWARD>;
+    static std::atomic<uint64_t> allowed;
+    const size_t smem = shared_bytes<VN, BACKWARD>(p.C);
+    if (smem > 40 << 10)
+        if (int rc = allow_shared_memory((const void *)kernel, &allowed)) return rc;
+    const int64_t tickets = 2 * (int64_t)p.chunks + (BACKWARD && p.dweight ? (p.C + AFFINE_CHANNELS - 1) / AFFINE_CHANNELS : 0);
+    launch_after(kernel, (unsigned)std::min<int64_t>(tickets, (BACKWARD ? 3 : 4) * num_sms()), NA_THREADS, smem, stream, p);
+    PCX_LAUNCH_CHECK();
+    return PCX_OK;
+}
+template <typename T, bool BACKWARD, int DROP>
+int run_act(const NormAct &p, cudaStream_t stream) {
+    if (p.act == ACT_RELU) return run_ring<T, ACT_RELU, DROP, BACKWARD>(p, stream);
+    if (p.act == ACT_SILU) return run_ring<T, ACT_SILU, DROP, BACKWARD>(p, stream);
+    if (p.act == ACT_GELU) return run_ring<T, ACT_GELU, DROP, BACKWARD>(p, stream);
+    return run_ring<T, ACT_NONE, DROP, BACKWARD>(p, stream);
+}
+template <typename T, bool BACKWARD>
+int run_lump(const NormAct &p, int vn, cudaStream_t stream) {
+    if (p.stages) return !p.drop.on ? run_act<T, BACKWARD, 0>(p, stream) : p.drop.state ? run_act<T, BACKWARD, 2>(p, stream) : run_act<T, BACKWARD, 1>(p, stream);
+    if (vn == 8) return run_kernel<T, 8, -1, -1, BACKWARD>(p, stream);
+    if (vn == 4) return run_kernel<T, 4, -1, -1, BACKWARD>(p, stream);
+    if (vn == 2) return run_kernel<T, 2, -1, -1, BACKWARD>(p, stream);
+    return run_kernel<T, 1, -1, -1, BACKWARD>(p, stream);
+}
+
+}  // namespace
+
+template <typename T>
+int norm_act_rows(const NormAct &p, int vn, bool backward, cudaStream_t stream) {
+    return backward ? run_lump<T, true>(p, vn, stream) : run_lump<T, false>(p, vn, stream);
+}
+#endif
+
+}  // namespace pcx

@@ -3,6 +3,7 @@
 // the thread layout (vector column, row lane) they share.
 #pragma once
 #include <initializer_list>
+#include <type_traits>
 
 #include "common.cuh"
 
@@ -105,9 +106,60 @@ struct Lump {
             *reinterpret_cast<uint16_t *>(p) = (uint16_t)w[0];
         }
     }
+    // What is not read again soon goes from the L2 first.
+    __device__ __forceinline__ void store_streaming(T *__restrict__ p) const {
+        static_assert(BYTES >= 16, "whole accesses");
+#pragma unroll
+        for (int q = 0; q < BYTES / 16; ++q) __stcs(reinterpret_cast<uint4 *>(p) + q, make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]));
+    }
     __device__ __forceinline__ float get(int i) const { return to_f32<T>(reinterpret_cast<const T *>(w)[i]); }
     __device__ __forceinline__ void set(int i, float v) { reinterpret_cast<T *>(w)[i] = from_f32<T>(v); }
 };
+
+// Channels are worked on in pairs: sm_100 has fp32 instructions for two at once.  (A lump of one channel is a pair with nothing behind.)
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(*reinterpret_cast<uint64_t *>(&a)), "l"(*reinterpret_cast<uint64_t *>(&b)), "l"(*reinterpret_cast<uint64_t *>(&c)));
+    return *reinterpret_cast<float2 *>(&d);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(*reinterpret_cast<uint64_t *>(&a)), "l"(*reinterpret_cast<uint64_t *>(&b)));
+    return *reinterpret_cast<float2 *>(&d);
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(*reinterpret_cast<uint64_t *>(&a)), "l"(*reinterpret_cast<uint64_t *>(&b)));
+    return *reinterpret_cast<float2 *>(&d);
+}
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+__device__ __forceinline__ float2 neg2(float2 v) { return make_float2(-v.x, -v.y); }
+
+template <typename T>
+__device__ __forceinline__ float2 unpack(uint32_t w);
+template <>
+__device__ __forceinline__ float2 unpack<__nv_bfloat16>(uint32_t w) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
+template <>
+__device__ __forceinline__ float2 unpack<__half>(uint32_t w) { return __half22float2(*reinterpret_cast<__half2 *>(&w)); }
+
+template <typename T, int VN>
+__device__ __forceinline__ float2 pair_of(const Lump<T, VN> &v, int j) {
+    if constexpr (sizeof(T) == 4) return make_float2(__uint_as_float(v.w[2 * j]), VN > 1 ? __uint_as_float(v.w[2 * j + (VN > 1)]) : 0.f);
+    else return unpack<T>(v.w[j]);
+}
+template <typename T, int VN>
+__device__ __forceinline__ void set_pair(Lump<T, VN> &v, int j, float2 f) {
+    if constexpr (sizeof(T) == 4) {
+        v.w[2 * j] = __float_as_uint(f.x);
+        if (VN > 1) v.w[2 * j + (VN > 1)] = __float_as_uint(f.y);
+    } else if constexpr (std::is_same<T, __half>::value) {
+        const __half2 h = __floats2half2_rn(f.x, f.y);
+        v.w[j] = *reinterpret_cast<const uint32_t *>(&h);
+    } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(f.x, f.y);
+        v.w[j] = *reinterpret_cast<const uint32_t *>(&h);
+    }
+}
 
 // max(v, 0) that hands a NaN on
 __device__ __forceinline__ float relu(float v) {
