@@ -15,7 +15,7 @@ namespace pcx {
 namespace {
 
 constexpr int DO_THREADS = 256;
-constexpr int DO_UNROLL = 4;                  // lumps a thread has in flight (by channel or sample)
+constexpr int DO_UNROLL = 2;                  // lumps a thread has in flight (by channel or sample)
 constexpr int DO_CALLS = 2;                   // of the generator, a thread (by element)
 constexpr int DO_CHUNK_BYTES = 16 << 10;      // of rows, a block of the units' kernel
 
@@ -116,7 +116,7 @@ __global__ void __launch_bounds__(DO_THREADS, 6) drop_elements_kernel(const __gr
 
 // By channels of a sample, or by samples: a block has `rows` consecutive rows, and goes through them sample by sample.
 template <typename T, int VN, bool BACKWARD, bool SAMPLES>
-__global__ void __launch_bounds__(DO_THREADS) drop_units_kernel(const __grid_constant__ DropArgs p) {
+__global__ void __launch_bounds__(DO_THREADS, 4) drop_units_kernel(const __grid_constant__ DropArgs p) {
     start_after_previous();
     const Philox<true> rng(p.drop);
     const T *x = static_cast<const T *>(p.x), *other = static_cast<const T *>(BACKWARD ? p.y_in : p.residual);

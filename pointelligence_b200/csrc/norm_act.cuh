@@ -101,11 +101,15 @@ __device__ __forceinline__ float rcp(float v) {
 // reciprocals a pair they, not the memory, would bound a pass over 16-bit rows.  v in 1 .. 2^62.
 __device__ __forceinline__ float2 rcp2(float2 v) { return mul2(both(rcp(v.x * v.y)), make_float2(v.y, v.x)); }
 
-// 1 / (1 + exp(-z)); below z = -43 it stays at 2^-62
-__device__ __forceinline__ float2 sigmoid2(float2 z) {
-    const float2 t = mul2(z, both(-1.4426950408889634f));
-    return rcp2(add2(both(1.f), make_float2(fminf(ex2(t.x), 0x1p62f), fminf(ex2(t.y), 0x1p62f))));
-}
+// exp(-z), 2^62 at most, and 1 / (1 + exp(-z)), which stays at 2^-62 below z = -43
+struct Sigmoid2 {
+    float2 e, s;
+    __device__ __forceinline__ explicit Sigmoid2(float2 z) {
+        const float2 t = mul2(z, both(-1.4426950408889634f));
+        e = make_float2(fminf(ex2(t.x), 0x1p62f), fminf(ex2(t.y), 0x1p62f));
+        s = rcp2(add2(both(1.f), e));
+    }
+};
 // The normal distribution's function and density, by formula 7.1.26 of Abramowitz and Stegun for erfc(|z| / sqrt 2) / 2 (off by at most
 // 7.5e-8, an ulp of fp32): one exponential serves both.
 __device__ __forceinline__ void normal2(float2 z, float2 &cdf, float2 &density) {
@@ -125,7 +129,7 @@ __device__ __forceinline__ void normal2(float2 z, float2 &cdf, float2 &density) 
 
 __device__ __forceinline__ float2 act2(int act, float2 z) {
     if (act == ACT_RELU) return make_float2(relu(z.x), relu(z.y));
-    if (act == ACT_SILU) return mul2(z, sigmoid2(z));
+    if (act == ACT_SILU) return mul2(z, Sigmoid2(z).s);
     if (act == ACT_GELU) {
         float2 cdf, density;
         normal2(z, cdf, density);
@@ -136,9 +140,9 @@ __device__ __forceinline__ float2 act2(int act, float2 z) {
 // g times the slope at z
 __device__ __forceinline__ float2 act2_backward(int act, float2 z, float2 g) {
     if (act == ACT_RELU) return make_float2(z.x > 0.f ? g.x : 0.f, z.y > 0.f ? g.y : 0.f);
-    if (act == ACT_SILU) {   // s (1 + z (1 - s)) = s + z s (1 - s)
-        const float2 s = sigmoid2(z), zs = mul2(z, s);
-        return mul2(g, add2(s, fma2(zs, neg2(s), zs)));
+    if (act == ACT_SILU) {   // s (1 + z (1 - s)), and 1 - s = e s
+        const Sigmoid2 v(z);
+        return mul2(g, fma2(mul2(z, v.s), mul2(v.e, v.s), v.s));
     }
     if (act == ACT_GELU) {
         float2 cdf, density;
@@ -213,10 +217,10 @@ __device__ __forceinline__ Records records_of(const float2 *at, int count, int64
 template <bool BACKWARD>
 struct RecordSums {
     static constexpr int AHEAD = 8;   // loads at once
-    float a = 0.f, b = 0.f, m2 = 0.f, k = 0.f;
+    float a = 0.f, b = 0.f, m2 = 0.f, k = 0.f, last = 0.f;
     __device__ __forceinline__ void add(const Records &r, int stride, int g, int q, int deep) {
         const float2 *at = r.at + g;
-        if constexpr (!BACKWARD) k = __ldcg(at).x;
+        if constexpr (!BACKWARD) k = __ldcg(at).x, last = __ldcg(at + (int64_t)(r.count - 1) * stride).x;
         for (int i = q; i < r.count; i += AHEAD * deep) {
             float2 v[AHEAD];
 #pragma unroll
@@ -233,9 +237,9 @@ struct RecordSums {
         }
     }
     // (mean, M2) of all rows, or the two sums; `each`: elements of a row
-    __device__ __forceinline__ float2 done(const Records &r, int stride, int g, float each) const {
+    __device__ __forceinline__ float2 done(const Records &r, float each) const {
         if constexpr (BACKWARD) return make_float2(a, b);
-        const float d = __ldcg(r.at + (int64_t)(r.count - 1) * stride + g).x - k, less = r.unit - r.last;   // the last one's rows are fewer
+        const float d = last - k, less = r.unit - r.last;   // the last one's rows are fewer
         const float sum = (r.unit * a - less * d) * each, squares = (r.unit * b - less * d * d) * each, off = sum / (r.all * each);
         return make_float2(k + off, fmaxf(m2 + squares - sum * off, 0.f));
     }
@@ -273,7 +277,7 @@ __device__ __forceinline__ void merge_groups(const NormAct &p, const Records &r,
                 }
         }
         if (g < groups && q == 0) {
-            const float2 v = sums.done(r, p.G, g, each);
+            const float2 v = sums.done(r, each);
             stats[g] = BACKWARD ? make_float2(v.x * inverse, v.y * inverse) : make_float2(v.x, 1.f / sqrtf(v.y * inverse + p.eps));
         }
         sync_workers();
@@ -631,7 +635,7 @@ __device__ __forceinline__ void merge_window(const NormAct &p, const Records &r,
     for (int g = Team::rank(); g < p.G; g += Team::SIZE) {
         RecordSums<BACKWARD> sums;
         sums.add(r, p.G, g, 0, 1);
-        to[g] = sums.done(r, p.G, g, (float)p.W);
+        to[g] = sums.done(r, (float)p.W);
     }
 }
 
