@@ -12,6 +12,11 @@ fp32 master weights, every norm -> (+ identity) -> ReLU tail runs as one fused
 kernel (``layers.norm.fused_layer_norm``), the shortcut projection (with its row gather at a
 stride) is a one-tap MVMR of the library instead of a ``Linear``, and every decoder stage rebuilds the submanifold triplets of its own
 cloud instead of inheriting the up-sampling layer's.
+
+Arguments beyond the reference's: ``norm_groups`` (group norms instead of layer norms), ``activation``, ``dropout`` (of elements,
+behind a block's first activation) and ``drop_path`` (of a block's branch, sample by sample); with their defaults
+nothing changes.  Norm, activation and dropout are one operator then (``layers.norm.fused_group_norm_act``), and drop path
+is one with the tail of the block (``layers.dropout.fused_dropout``).
 """
 from __future__ import annotations
 
@@ -26,8 +31,9 @@ from torch import Tensor
 
 from . import _cabi
 from .internals.triplet_cache import triplet_cache_scope
-from .layers import MetaData, PointConv3d, RaggedLayerNorm, Upsample
-from .layers.norm import fused_layer_norm
+from .layers import MetaData, PointConv3d, RaggedGroupNorm, RaggedLayerNorm, Upsample
+from .layers.dropout import fused_dropout
+from .layers.norm import ACTIVATIONS, fused_group_norm_act, fused_layer_norm
 from .layers.triplets import (build_triplets_segmented, handle_stride_and_build_triplets,
                               radius_scaler_for_kernel_size)
 from .sparse_engines.tig import _takes_host_path
@@ -135,27 +141,36 @@ def project_rows(x: Tensor, rows, weight: Tensor) -> Tensor:
     return tig_mvmr(w, x.contiguous(), TigIndex.from_flat(scatter, gather, seg, n_out, x.shape[0], 1, True, rows is None))
 
 
-def _norm_act(norm: RaggedLayerNorm, x: Tensor, lengths: Tensor, residual=None, relu=True) -> Tensor:
-    return fused_layer_norm(x, lengths, norm.weight, norm.bias, norm.eps, residual=residual, relu=relu)
+def _norm_act(norm, x: Tensor, lengths: Tensor, residual=None, activation="relu", dropout=0.0) -> Tensor:
+    """``dropout(activation(norm(x) (+ residual)))``: the fused layer norm where that has it all, the grouped one otherwise."""
+    if norm.norm_type == "layer" and activation in ("relu", "identity") and dropout == 0.0:
+        return fused_layer_norm(x, lengths, norm.weight, norm.bias, norm.eps, residual=residual, relu=activation == "relu")
+    return fused_group_norm_act(x, lengths, norm._groups(), norm.weight, norm.bias, norm.eps, residual, activation, dropout)
+
+
+def _norm(planes: int, groups):
+    return RaggedLayerNorm(planes) if groups is None else RaggedGroupNorm(groups, planes)
 
 
 class BasicBlock(nn.Module):
-    def __init__(self, inplanes: int, planes: int, stride: float = 1.0):
+    def __init__(self, inplanes: int, planes: int, stride: float = 1.0, norm_groups=None, activation: str = "relu",
+                 dropout: float = 0.0, drop_path: float = 0.0):
         super().__init__()
         self.conv1 = Bf16PointConv3d(inplanes, planes, kernel_size=3, bias=False)
-        self.bn1 = RaggedLayerNorm(planes)
+        self.bn1 = _norm(planes, norm_groups)
         self.conv2 = Bf16PointConv3d(planes, planes, kernel_size=3, bias=False)
-        self.bn2 = RaggedLayerNorm(planes)
+        self.bn2 = _norm(planes, norm_groups)
         self.stride = stride
+        self.activation, self.dropout, self.drop_path = activation, dropout, drop_path
         self.shortcut = None
         if inplanes != planes:
             self.shortcut = nn.Linear(inplanes, planes, bias=False)
-            self.shortcut_norm = RaggedLayerNorm(planes)
+            self.shortcut_norm = _norm(planes, norm_groups)
 
     def forward(self, x: Tensor, m: MetaData) -> Tuple[Tensor, MetaData]:
         identity = x
         x, m = self._strided(x, m)
-        x = _norm_act(self.bn1, x, m.sample_sizes)
+        x = _norm_act(self.bn1, x, m.sample_sizes, activation=self.activation, dropout=self.dropout if self.training else 0.0)
         if self.stride != 1.0:
             scaler = radius_scaler_for_kernel_size(kernel_size=3, receptive_field_scaler=RFS)
             m.i, m.j, m.k, m.seg_offs, _ = build_triplets_segmented(
@@ -165,10 +180,17 @@ class BasicBlock(nn.Module):
         rows = m.downsample_indices if self.stride != 1.0 else None
         if self.shortcut is not None:
             identity = project_rows(identity, rows, self.shortcut.weight)
-            identity = _norm_act(self.shortcut_norm, identity, m.sample_sizes, relu=False)
+            identity = _norm_act(self.shortcut_norm, identity, m.sample_sizes, activation="identity")
         elif rows is not None:
             identity = identity[rows]
-        return _norm_act(self.bn2, x, m.sample_sizes, residual=identity), m
+        return self._tail(x, identity, m.sample_sizes), m
+
+    def _tail(self, x: Tensor, identity: Tensor, lengths: Tensor) -> Tensor:
+        if not (self.training and self.drop_path > 0.0):
+            return _norm_act(self.bn2, x, lengths, residual=identity, activation=self.activation)
+        x = _norm_act(self.bn2, x, lengths, activation="identity")
+        x = fused_dropout(x, self.drop_path, unit="sample", lengths=lengths, residual=identity, relu=self.activation == "relu")
+        return {"silu": F.silu, "gelu": F.gelu}[self.activation](x) if self.activation in ("silu", "gelu") else x
 
     def _strided(self, x, m):
         m = handle_stride_and_build_triplets(m, self.stride, self.conv1.kernel_size_3, RFS)
@@ -187,28 +209,34 @@ class UpsampleBf16(Upsample):
 
 class ResUNet(nn.Module):
     def __init__(self, in_channels=3, num_classes=20, base_channels=32, channels: Sequence[int] = (32, 64, 128, 256),
-                 tr_channels: Sequence[int] = (96, 96, 128, 256), layers: Sequence[int] = (2,) * 8):
+                 tr_channels: Sequence[int] = (96, 96, 128, 256), layers: Sequence[int] = (2,) * 8, norm_groups=None,
+                 activation: str = "relu", dropout: float = 0.0, drop_path: float = 0.0):
         super().__init__()
+        if activation not in ACTIVATIONS:
+            raise ValueError(f"activation is one of {sorted(ACTIVATIONS)}, got {activation!r}")
+        if not (0.0 <= dropout <= 1.0 and 0.0 <= drop_path <= 1.0):
+            raise ValueError(f"dropout probabilities have to be between 0 and 1, but got {dropout} and {drop_path}")
         C, TR, L = list(channels), list(tr_channels), list(layers)
+        self.activation = activation
         self.conv1 = Bf16PointConv3d(in_channels, base_channels, kernel_size=5, bias=False)
-        self.norm1 = RaggedLayerNorm(base_channels)
+        self.norm1 = _norm(base_channels, norm_groups)
 
         def stage(cin, cout, n, stride):
-            return nn.ModuleList([BasicBlock(cin if b == 0 else cout, cout, stride if b == 0 else 1.0)
-                                  for b in range(n)])
+            return nn.ModuleList([BasicBlock(cin if b == 0 else cout, cout, stride if b == 0 else 1.0, norm_groups, activation,
+                                             dropout, drop_path) for b in range(n)])
 
         self.block1 = stage(base_channels, C[0], L[0], 1.0)
         self.enc_block1 = stage(C[0], C[1], L[1], 2.0)
         self.enc_block2 = stage(C[1], C[2], L[2], 2.0)
         self.enc_block3 = stage(C[2], C[3], L[3], 2.0)
         self.upsample4 = UpsampleBf16(C[3], TR[3], kernel_size=3, bias=False, receptive_field_scaler=RFS)
-        self.norm4_tr = RaggedLayerNorm(TR[3])
+        self.norm4_tr = _norm(TR[3], norm_groups)
         self.block4_tr = stage(TR[3], TR[3], L[4], 1.0)
         self.upsample3 = UpsampleBf16(C[2] + TR[3], TR[2], kernel_size=3, bias=False, receptive_field_scaler=RFS)
-        self.norm3_tr = RaggedLayerNorm(TR[2])
+        self.norm3_tr = _norm(TR[2], norm_groups)
         self.block3_tr = stage(TR[2], TR[2], L[5], 1.0)
         self.upsample2 = UpsampleBf16(C[1] + TR[2], TR[1], kernel_size=3, bias=False, receptive_field_scaler=RFS)
-        self.norm2_tr = RaggedLayerNorm(TR[1])
+        self.norm2_tr = _norm(TR[1], norm_groups)
         self.block2_tr = stage(TR[1], TR[1], L[6], 1.0)
         self.block1_tr = stage(C[0] + TR[1], TR[0], L[7], 1.0)
         self.final_conv = Bf16PointConv3d(TR[0], num_classes, kernel_size=1, bias=True)
@@ -231,7 +259,7 @@ class ResUNet(nn.Module):
         m = handle_stride_and_build_triplets(m, 1.0, self.conv1.kernel_size_3, RFS)
         x = self.conv1(feat, m.i, m.j, m.k, m.num_points(), contract=m.contract, seg_offs=m.seg_offs)
         m.dirty_triplets()
-        x = _norm_act(self.norm1, x, m.sample_sizes)
+        x = _norm_act(self.norm1, x, m.sample_sizes, activation=self.activation)
         for blk in self.block1:
             x, m = blk(x, m)
         skips: List[Tensor] = [x]
@@ -243,17 +271,17 @@ class ResUNet(nn.Module):
         # convolve over the submanifold neighbourhoods of their own cloud
         x, m = self.upsample4(skips[-1], m)
         m.dirty_triplets()
-        x = _norm_act(self.norm4_tr, x, m.sample_sizes)
+        x = _norm_act(self.norm4_tr, x, m.sample_sizes, activation=self.activation)
         for blk in self.block4_tr:
             x, m = blk(x, m)
         x, m = self.upsample3(torch.cat([skips[-2], x], dim=1), m)
         m.dirty_triplets()
-        x = _norm_act(self.norm3_tr, x, m.sample_sizes)
+        x = _norm_act(self.norm3_tr, x, m.sample_sizes, activation=self.activation)
         for blk in self.block3_tr:
             x, m = blk(x, m)
         x, m = self.upsample2(torch.cat([skips[-3], x], dim=1), m)
         m.dirty_triplets()
-        x = _norm_act(self.norm2_tr, x, m.sample_sizes)
+        x = _norm_act(self.norm2_tr, x, m.sample_sizes, activation=self.activation)
         for blk in self.block2_tr:
             x, m = blk(x, m)
         x = torch.cat([skips[0], x], dim=1)

@@ -124,3 +124,13 @@ def test_module_without_training_is_the_tail_alone():
     assert layer(x) is x and torch.equal(layer(x, residual=res, relu=True), (x + res).relu())
     assert RaggedDropout(0.0)(x) is x
     assert "p=0.5" in repr(layer)
+
+
+def test_network_arguments():
+    from pointelligence_b200.backbone import ResUNet
+
+    plain, grouped = ResUNet(), ResUNet(norm_groups=8, activation="silu", dropout=0.1, drop_path=0.2)
+    assert {k: v.shape for k, v in plain.state_dict().items()} == {k: v.shape for k, v in grouped.state_dict().items()}
+    for bad in (dict(activation="tanh"), dict(dropout=1.5), dict(drop_path=-0.1), dict(norm_groups=7)):
+        with pytest.raises(ValueError):
+            ResUNet(**bad)
