@@ -457,7 +457,7 @@ int pcx_ragged_group_norm_backward(const void *d_grad_y, const void *d_x,
  * G = 1 is the ragged layer norm, G = C the instance norm; C <= 65536.
  * `activation`: a pcx_activation.  `dropout` is the probability of the dropout
  * by element described at pcx_dropout (0: none).  d_weight / d_bias (fp32, C) may both
- * be null, and so may d_residual.  d_mean / d_rstd (fp32, S * G, index s * G + g)
+ * be null, and so may d_residual.  d_mean / d_rstd (fp64, S * G, index s * G + g)
  * are outputs kept for the backward pass, which makes the activation's argument and the
  * mask again: give it the tensors, the probability and the seed of the forward
  * call.  d_grad_weight / d_grad_bias (fp32, C) may both be null, and so may
@@ -475,15 +475,15 @@ size_t pcx_ragged_group_norm_act_workspace_bytes(int64_t N, int64_t S, int C,
                                                  int G, int dtype);
 int pcx_ragged_group_norm_act(const void *d_x, const int64_t *d_lengths,
                               const float *d_weight, const float *d_bias,
-                              const void *d_residual, void *d_y, float *d_mean,
-                              float *d_rstd, int64_t N, int64_t S, int C, int G,
+                              const void *d_residual, void *d_y, double *d_mean,
+                              double *d_rstd, int64_t N, int64_t S, int C, int G,
                               double eps, int activation, double dropout,
                               uint64_t seed, uint64_t offset, const int64_t *d_rng,
                               int dtype, void *d_ws, size_t ws_bytes, void *stream);
 int pcx_ragged_group_norm_act_backward(
     const void *d_grad_y, const void *d_x, const void *d_residual,
     const int64_t *d_lengths, const float *d_weight, const float *d_bias,
-    const float *d_mean, const float *d_rstd, void *d_grad_x, float *d_grad_weight,
+    const double *d_mean, const double *d_rstd, void *d_grad_x, float *d_grad_weight,
     float *d_grad_bias, void *d_grad_residual, int64_t N, int64_t S, int C, int G,
     int activation, double dropout, uint64_t seed, uint64_t offset,
     const int64_t *d_rng, int dtype, void *d_ws, size_t ws_bytes, void *stream);

@@ -668,11 +668,11 @@ std::tuple<Tensor, Tensor, Tensor> group_norm_act_forward(Tensor x, const Tensor
     const Tensor residual = residual_ ? residual_->to(x.scalar_type()).contiguous() : Tensor();
     const int64_t S = lengths.numel();
     Tensor y = at::empty_like(x);
-    Tensor stats = at::empty({2, S * t.groups}, x.options().dtype(at::kFloat));
+    Tensor stats = at::empty({2, S * t.groups}, x.options().dtype(at::kDouble));
     Tensor mean = stats.select(0, 0), rstd = stats.select(0, 1);
     Tensor ws = workspace(pcx_ragged_group_norm_act_workspace_bytes(N, S, (int)C, (int)t.groups, code), x);
     check(pcx_ragged_group_norm_act(ptr(x), ptr_as<int64_t>(lengths), ptr_as<float>(weight), ptr_as<float>(bias), ptr(residual), ptr(y),
-                                    ptr_as<float>(mean), ptr_as<float>(rstd), N, S, (int)C, (int)t.groups, t.eps, (int)t.activation, t.dropout, t.seed,
+                                    ptr_as<double>(mean), ptr_as<double>(rstd), N, S, (int)C, (int)t.groups, t.eps, (int)t.activation, t.dropout, t.seed,
                                     t.offset, state ? ptr_as<int64_t>(*state) : nullptr, code, ptr(ws), ws.numel(), stream()));
     return {y, mean, rstd};
 }
@@ -717,7 +717,7 @@ struct GroupNormAct : public torch::autograd::Function<GroupNormAct> {
         if (needs(2)) gres = at::empty_like(x);
         Tensor ws = workspace(pcx_ragged_group_norm_act_workspace_bytes(N, S, (int)C, (int)sizes[0], code), x);
         check(pcx_ragged_group_norm_act_backward(ptr(grad_y), ptr(x), ptr(residual), ptr_as<int64_t>(lengths), ptr_as<float>(weight),
-                                                 ptr_as<float>(bias), ptr_as<float>(saved[6]), ptr_as<float>(saved[7]), ptr(gx), ptr_as<float>(gw),
+                                                 ptr_as<float>(bias), ptr_as<double>(saved[6]), ptr_as<double>(saved[7]), ptr(gx), ptr_as<float>(gw),
                                                  ptr_as<float>(gb), ptr(gres), N, S, (int)C, (int)sizes[0], (int)sizes[1],
                                                  ctx->saved_data["dropout"].toDouble(), (uint64_t)sizes[2], (uint64_t)sizes[3],
                                                  ptr_as<int64_t>(saved[5]), code, ptr(ws), ws.numel(), stream()));

@@ -15,7 +15,7 @@ constexpr int NA_CHUNK_BYTES = 96 << 10;        // of x
 constexpr int NA_STAGE_BYTES = 24 << 10;        // of a tile, all tensors
 constexpr int NA_RING_BYTES = 110 << 10;        // of shared memory, a block: two on a multiprocessor
 constexpr int NA_MAX_C = 1 << 16;
-constexpr int NA_RECORDS = 16 << 10;            // of groups that a block reads for itself, at most: 128 KB where all rows are one sample's
+constexpr int NA_RECORDS = 8 << 10;             // of groups that a block reads for itself, at most: 128 KB where all rows are one sample's
 constexpr int64_t NA_LAG_BYTES = 64 << 20;      // of x, and of the gradient
 
 // ------------------------------------------------------------ the samples' rows ----
@@ -75,7 +75,7 @@ __global__ void __launch_bounds__(OFFSETS_THREADS) na_layout_kernel(const int64_
         p.spans[s] = v;
         if (hi > lo) windows += windows_of(p, v);
         if (!BACKWARD && hi == lo)
-            for (int g = 0; g < p.G; ++g) p.mean[s * p.G + g] = 0.f, p.rstd[s * p.G + g] = 1.f / sqrtf(p.eps);
+            for (int g = 0; g < p.G; ++g) p.mean[s * p.G + g] = 0.0, p.rstd[s * p.G + g] = 1.0 / sqrt(p.eps);
         if (BACKWARD && p.dweight && (hi == lo || hi % p.rows == 0))   // behind a sample that ends with a chunk, and for one without rows, a number is left out
             for (int c = 0; c < p.C; ++c) p.rec[(hi / p.rows + s) * p.C + c] = make_float2(0.f, 0.f);
     }
@@ -102,8 +102,8 @@ size_t carve(void *ws, int64_t N, int64_t S, int C, int G, int dtype, NormAct *o
     p.rec = c.take<float2>((size_t)(p.chunks + S) * C);
     p.window = (int)std::max<int64_t>(1, (p.chunks * (int64_t)G + NA_RECORDS - 1) / NA_RECORDS);
     const size_t windows = p.window > 1 ? (size_t)windows_in_all(p.chunks, S, p.window) : 0;
-    p.of_piece = c.take<float2>((size_t)(p.chunks + S) * G);
-    p.of_window = windows ? c.take<float2>(windows * G) : p.of_piece;
+    p.of_piece = c.take<float4>((size_t)(p.chunks + S) * G);   // (backward: of float2)
+    p.of_window = windows ? c.take<float4>(windows * G) : p.of_piece;
     p.control = c.take<int>(CONTROL_WORDS + (size_t)S + windows);
     if (out) *out = p;
     return c.off;
@@ -128,7 +128,7 @@ int run(const int64_t *d_lengths, NormAct &p, int dtype, int vn, int activation,
         p.tile_rows = lanes * std::max(1, NA_STAGE_BYTES / (lanes * row_bytes * tensors));
         p.sums_tile_rows = BACKWARD ? p.tile_rows : p.tile_rows * tensors;
         p.stage_bytes = (p.tile_rows * row_bytes * tensors + 127) / 128 * 128;
-        p.stages = std::min(RING_STAGES, (NA_RING_BYTES - (int)ring_bytes(p.C, BACKWARD)) / p.stage_bytes);
+        p.stages = std::min(RING_STAGES, (NA_RING_BYTES - (int)ring_bytes(p.C, p.G, BACKWARD)) / p.stage_bytes);
         if (p.stages < 2) p.stages = 0;
     }
     launch_after(na_layout_kernel<BACKWARD>, 1, p.S <= 256 ? 256 : OFFSETS_THREADS, 0, stream, d_lengths, p);
@@ -164,7 +164,7 @@ size_t pcx_ragged_group_norm_act_workspace_bytes(int64_t N, int64_t S, int C, in
 }
 
 int pcx_ragged_group_norm_act(const void *d_x, const int64_t *d_lengths, const float *d_weight, const float *d_bias, const void *d_residual, void *d_y,
-                              float *d_mean, float *d_rstd, int64_t N, int64_t S, int C, int G, double eps, int activation, double dropout, uint64_t seed,
+                              double *d_mean, double *d_rstd, int64_t N, int64_t S, int C, int G, double eps, int activation, double dropout, uint64_t seed,
                               uint64_t offset, const int64_t *d_rng, int dtype, void *d_ws, size_t ws_bytes, void *stream_) {
     cudaStream_t stream = (cudaStream_t)stream_;
     if (!sizes_ok(N, S, C, G, dtype, activation))
@@ -177,7 +177,7 @@ int pcx_ragged_group_norm_act(const void *d_x, const int64_t *d_lengths, const f
     const size_t need = carve(d_ws, N, S, C, G, dtype, &p);
     if (ws_bytes < need) PCX_FAIL(PCX_E_CAPACITY, "pcx_ragged_group_norm_act: workspace %zu < %zu bytes", ws_bytes, need);
     p.x = d_x, p.residual = d_residual, p.y = d_y, p.weight = d_weight, p.bias = d_bias, p.mean = d_mean, p.rstd = d_rstd;
-    p.N = N, p.S = S, p.C = C, p.G = G, p.W = C / G, p.by_width = (uint32_t)((0xFFFFFFFFull + p.W) / p.W), p.eps = (float)eps;
+    p.N = N, p.S = S, p.C = C, p.G = G, p.W = C / G, p.by_width = (uint32_t)((0xFFFFFFFFull + p.W) / p.W), p.eps = eps;
     const int vn = lump_of(C, dtype, {d_x, d_residual, d_y});
     prof_begin("group_norm_act(fwd)", stream);
     const int rc = run<false>(d_lengths, p, dtype, vn, activation, stream);
@@ -186,7 +186,7 @@ int pcx_ragged_group_norm_act(const void *d_x, const int64_t *d_lengths, const f
 }
 
 int pcx_ragged_group_norm_act_backward(const void *d_grad_y, const void *d_x, const void *d_residual, const int64_t *d_lengths, const float *d_weight,
-                                       const float *d_bias, const float *d_mean, const float *d_rstd, void *d_grad_x, float *d_grad_weight,
+                                       const float *d_bias, const double *d_mean, const double *d_rstd, void *d_grad_x, float *d_grad_weight,
                                        float *d_grad_bias, void *d_grad_residual, int64_t N, int64_t S, int C, int G, int activation, double dropout,
                                        uint64_t seed, uint64_t offset, const int64_t *d_rng, int dtype, void *d_ws, size_t ws_bytes, void *stream_) {
     cudaStream_t stream = (cudaStream_t)stream_;
@@ -202,7 +202,7 @@ int pcx_ragged_group_norm_act_backward(const void *d_grad_y, const void *d_x, co
     const size_t need = carve(d_ws, N, S, C, G, dtype, &p);
     if (ws_bytes < need) PCX_FAIL(PCX_E_CAPACITY, "pcx_ragged_group_norm_act_backward: workspace %zu < %zu bytes", ws_bytes, need);
     p.x = d_x, p.residual = d_residual, p.g = d_grad_y, p.dx = d_grad_x, p.dresidual = d_grad_residual, p.weight = d_weight, p.bias = d_bias;
-    p.mean = const_cast<float *>(d_mean), p.rstd = const_cast<float *>(d_rstd), p.dweight = d_grad_weight, p.dbias = d_grad_bias;
+    p.mean = const_cast<double *>(d_mean), p.rstd = const_cast<double *>(d_rstd), p.dweight = d_grad_weight, p.dbias = d_grad_bias;
     p.N = N, p.S = S, p.C = C, p.G = G, p.W = C / G, p.by_width = (uint32_t)((0xFFFFFFFFull + p.W) / p.W);
     const int vn = lump_of(C, dtype, {d_x, d_residual, d_grad_y, d_grad_x, d_grad_residual});
     prof_begin("group_norm_act(bwd)", stream);

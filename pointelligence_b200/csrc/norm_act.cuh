@@ -26,8 +26,8 @@
 // Tickets are ordered so that a sample is applied some chunks after its sums, in the hope that the wait for them is over by then.
 //
 // What is summed:
-//   forward   mean and sum of squares about it.  A block sums x - k and its square, k the channel's value in the piece's first row:
-//             as k is one of the n summed values, (k - mean)^2 is at most their sum of squares M2, and what cancels in
+//   forward   mean and sum of squares about it.  A block sums x - k and its square, k the channel's value in the piece's first row
+//             (or next to it, see shift_of): as k is one of the n summed values, (k - mean)^2 is at most their sum of squares M2, and what cancels in
 //             sum (x - k)^2 - n (mean - k)^2 is at most (n + 1) M2: n + 1 roundings at worst, one where rows are alike.
 //   backward  gz and gz * xh.
 #pragma once
@@ -54,19 +54,19 @@ struct NormAct {
     const void *x, *residual, *g;
     void *y, *dx, *dresidual;
     const float *weight, *bias;
-    float *mean, *rstd;            // (S, G)
+    double *mean, *rstd;           // (S, G)
     float *dweight, *dbias;
     int64_t *offsets;              // (S + 1)
     Span *spans;                   // (S)
     float2 *rec;                   // (pieces, C): mean and M2; or sums of gz and gz * xh
-    float2 *of_piece, *of_window;  // (pieces, G), (windows, G): the same of groups, the sums with the channels' weights
+    void *of_piece, *of_window;    // (pieces, G), (windows, G) of Record: the same of groups, the sums with the channels' weights
     int *control;                  // the words above, then windows that each sample has, pieces that each window has
     unsigned int *status;
     int64_t N, S;
     int C, G, W, rows, chunks, window, lag, act;
     int tile_rows, sums_tile_rows, stages, stage_bytes;   // of the ring
     uint32_t by_width;             // c / W = c * by_width >> 32 (c * W < 2^32); W = 1: c
-    float eps;
+    double eps;
     Dropping drop;
 };
 
@@ -201,60 +201,108 @@ __device__ __forceinline__ bool sync_workers_and(bool v) {
     return all != 0;
 }
 
-// Records that follow one another: `count` of `unit` rows each, but for the first and the last.
-struct Records {
-    const float2 *at;
-    int count;
-    float first, unit, last, all;   // rows
-};
-// Rows lo .. hi by spans of `unit` rows, the first of which begins at `from`.
-__device__ __forceinline__ Records records_of(const float2 *at, int count, int64_t lo, int64_t hi, int64_t from, int64_t unit) {
-    return {at, count, (float)(min(hi, from + unit) - lo), (float)unit, (float)(hi - (from + (count - 1) * unit)), (float)(hi - lo)};
+// What a piece leaves of a group.  Forward: mean and M2, the mean in two floats: rounded to one, it would make the activation's argument
+// uncertain by 2^-25 of it, and with it the sign that decides the ReLU's gradient: of 70 million elements about one came out on the
+// other side, each of which moves dbias by a whole gradient.  (Roundings further down are many, and average out.)
+template <bool BACKWARD>
+struct Record;
+template <>
+struct __align__(16) Record<false> { float mean, low, m2, none; };
+template <>
+struct __align__(8) Record<true> { float x, y; };
+__device__ __forceinline__ Record<true> load_record(const Record<true> *p) {
+    const float2 v = __ldcg(reinterpret_cast<const float2 *>(p));
+    return {v.x, v.y};
+}
+__device__ __forceinline__ Record<false> load_record(const Record<false> *p) {
+    const float4 v = __ldcg(reinterpret_cast<const float4 *>(p));
+    return {v.x, v.y, v.z, 0.f};
 }
 
-// Sums over records, of which a thread has some.  Forward, with d a record's mean less the first one's (so that their differences, not the means, are rounded; the first's own
-// is zero, whatever its rows): of d, d^2 and M2.  Backward: of both sums.
+// Records that follow one another: `count` of `unit` rows each, but for the first and the last.
 template <bool BACKWARD>
-struct RecordSums {
+struct Records {
+    const Record<BACKWARD> *at;
+    int count;
+    float first, unit, last;   // rows
+    double inverse;            // 1 / elements of all of them
+};
+// Rows lo .. hi by spans of `unit` rows, the first of which begins at `from`; `each` elements a row.
+template <bool BACKWARD>
+__device__ __forceinline__ Records<BACKWARD> records_of(const void *at, int64_t first, int count, int64_t lo, int64_t hi, int64_t from, int64_t unit, int each) {
+    return {static_cast<const Record<BACKWARD> *>(at) + first, count, (float)(min(hi, from + unit) - lo), (float)unit, (float)(hi - (from + (count - 1) * unit)),
+            1.0 / ((double)(hi - lo) * each)};
+}
+
+// Sums over records, of which a thread has some.  Forward all are differences from the first record, or squares of them, so that what
+// is rounded is small: a, b of means and their squares, m2 of M2.  Backward: of both sums.
+template <bool BACKWARD>
+struct RecordSums;
+template <>
+struct RecordSums<true> {
     static constexpr int AHEAD = 8;   // loads at once
-    float a = 0.f, b = 0.f, m2 = 0.f, k = 0.f, last = 0.f;
-    __device__ __forceinline__ void add(const Records &r, int stride, int g, int q, int deep) {
-        const float2 *at = r.at + g;
-        if constexpr (!BACKWARD) k = __ldcg(at).x, last = __ldcg(at + (int64_t)(r.count - 1) * stride).x;
+    float a = 0.f, b = 0.f, m2 = 0.f;
+    __device__ __forceinline__ void add(const Records<true> &r, int stride, int g, int q, int deep) {
+        const Record<true> *at = r.at + g;
         for (int i = q; i < r.count; i += AHEAD * deep) {
-            float2 v[AHEAD];
+            Record<true> v[AHEAD];
 #pragma unroll
-            for (int u = 0; u < AHEAD; ++u) v[u] = i + u * deep < r.count ? __ldcg(at + (int64_t)(i + u * deep) * stride) : make_float2(BACKWARD ? 0.f : k, 0.f);
+            for (int u = 0; u < AHEAD; ++u) v[u] = i + u * deep < r.count ? load_record(at + (int64_t)(i + u * deep) * stride) : Record<true>{0.f, 0.f};
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u) a += v[u].x, b += v[u].y;
+        }
+    }
+    __device__ __forceinline__ Record<true> done(const Records<true> &, int) const { return {a, b}; }
+};
+template <>
+struct RecordSums<false> {
+    static constexpr int AHEAD = 8;
+    float a = 0.f, b = 0.f, m2 = 0.f;
+    Record<false> k, last;
+    __device__ __forceinline__ float away(const Record<false> &v) const { return (v.mean - k.mean) + (v.low - k.low); }
+    __device__ __forceinline__ void add(const Records<false> &r, int stride, int g, int q, int deep) {
+        const Record<false> *at = r.at + g;
+        k = load_record(at), last = load_record(at + (int64_t)(r.count - 1) * stride);
+        for (int i = q; i < r.count; i += AHEAD * deep) {
+            Record<false> v[AHEAD];
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u) v[u] = i + u * deep < r.count ? load_record(at + (int64_t)(i + u * deep) * stride) : k;
 #pragma unroll
             for (int u = 0; u < AHEAD; ++u) {
-                if constexpr (BACKWARD) {
-                    a += v[u].x, b += v[u].y;
-                } else {
-                    const float d = v[u].x - k;
-                    a += d, b += d * d, m2 += v[u].y;
-                }
+                const float d = away(v[u]);
+                a += d, b += d * d, m2 += v[u].m2 - k.m2;
             }
         }
     }
-    // (mean, M2) of all rows, or the two sums; `each`: elements of a row
-    __device__ __forceinline__ float2 done(const Records &r, float each) const {
-        if constexpr (BACKWARD) return make_float2(a, b);
-        const float d = last - k, less = r.unit - r.last;   // the last one's rows are fewer
-        const float sum = (r.unit * a - less * d) * each, squares = (r.unit * b - less * d * d) * each, off = sum / (r.all * each);
-        return make_float2(k + off, fmaxf(m2 + squares - sum * off, 0.f));
+    struct Moments { double mean, m2; };
+    __device__ __forceinline__ Moments moments(const Records<false> &r, int each) const {   // (the first record's rows do not matter to a and b, the last's do)
+        const double d = away(last), less = (double)r.unit - r.last;
+        const double sum = ((double)r.unit * a - less * d) * each, off = sum * r.inverse;
+        const double squares = ((double)r.unit * b - less * d * d) * each - sum * off;
+        return {((double)k.mean + k.low) + off, fmax(((double)r.count * k.m2 + m2) + squares, 0.0)};
+    }
+    __device__ __forceinline__ Record<false> done(const Records<false> &r, int each) const {
+        const Moments v = moments(r, each);
+        return {(float)v.mean, (float)(v.mean - (double)(float)v.mean), (float)v.m2, 0.f};
     }
 };
+
+// 1 / sqrt(v), from fp32's by a step of Newton's
+__device__ __forceinline__ double rsqrt_of(double v) {
+    const double y = rsqrtf((float)v);
+    return y * (1.5 - 0.5 * v * y * y);
+}
 
 // What a second pass needs of the groups that channels c0 .. c1 - 1 are in, from the sample's records, into `stats` (shared memory) by all
 // workers: mean and rstd, or the backward's two means.  Every block does this for itself, with the sample's windows counted: a block
 // that did it for all would keep them waiting for one more turn through the L2.  Threads stand side by side on the groups and, where
 // there are fewer of them, in rows on the records.
+struct Stats { double x, y; };
 template <bool BACKWARD>
-__device__ __forceinline__ void merge_groups(const NormAct &p, const Records &r, int groups, float2 *stats, float4 *scratch) {
-    const float each = (float)p.W, inverse = 1.f / (r.all * each);
+__device__ __forceinline__ void merge_groups(const NormAct &p, const Records<BACKWARD> &r, int groups, Stats *stats, float4 *scratch) {
     const int wide = min(groups, NA_THREADS), at = threadIdx.x % wide, q = threadIdx.x / wide;
     const bool shuffles = wide < 32 && 32 % wide == 0;
-    int deep = NA_THREADS / wide;
+    const int deep = NA_THREADS / wide;
     for (int base = 0; base < groups; base += wide) {
         const int g = base + at;
         RecordSums<BACKWARD> sums;
@@ -277,8 +325,12 @@ __device__ __forceinline__ void merge_groups(const NormAct &p, const Records &r,
                 }
         }
         if (g < groups && q == 0) {
-            const float2 v = sums.done(r, each);
-            stats[g] = BACKWARD ? make_float2(v.x * inverse, v.y * inverse) : make_float2(v.x, 1.f / sqrtf(v.y * inverse + p.eps));
+            if constexpr (BACKWARD) {
+                stats[g] = {sums.a * r.inverse, sums.b * r.inverse};
+            } else {
+                const auto v = sums.moments(r, p.W);
+                stats[g] = {v.mean, rsqrt_of(v.m2 * r.inverse + p.eps)};
+            }
         }
         sync_workers();
     }
@@ -310,12 +362,12 @@ __device__ __forceinline__ bool wait_for(const int *word, int value, unsigned in
 // Forward z = x a + b, with the mean in b: that rounds z by 2^-24 of |mean| / deviation more, as the mean's own rounding does.  Backward
 // z = (x - mu) a + b, as sums of gz (x - mu) want the difference, and dx = gz a - m1 - (x - mu) m2.
 enum { K_A = 0, K_B = 1, K_MU = 2, K_M1 = 3, K_M2 = 4 };
-template <int VN>
+template <int VN, bool BACKWARD>
 struct Constants {
     static constexpr int QUAD = VN < 4 ? VN : 4, PAIRS = QUAD < 2 ? 1 : QUAD / 2, QUADS = VN / QUAD;
     float *at;
-    float2 *stats;             // of the second pass: the groups'
-    float4 *scratch;           // an entry a thread
+    Stats *stats;              // of the second pass: the groups'
+    float4 *scratch;           // of merge_groups
     int64_t s = -1;            // whose they are
     int pass = -1;
     __device__ __forceinline__ void read(const Columns &l, int k, int h, float2 *out) const {
@@ -335,19 +387,18 @@ struct Constants {
         }
     }
     // By all workers, once they have met.  `second`: of the second pass, for which the sample's records are waited for; false: in vain.
-    template <bool BACKWARD>
     __device__ __forceinline__ bool load(const NormAct &p, const Columns &l, int64_t s_, int pass_, bool second) {
         const int c0 = pass_ * l.cols * VN, c1 = min(p.C, c0 + l.cols * VN), g0 = group_of(p, c0);
         float w = 1.f, bias = 0.f, mu = 0.f, rs = 0.f;   // of the thread's first channel: read before the wait
         const auto known = [&](int c) {
             if (p.weight) w = __ldg(p.weight + c), bias = __ldg(p.bias + c);
-            if (BACKWARD) mu = __ldg(p.mean + s_ * p.G + group_of(p, c)), rs = __ldg(p.rstd + s_ * p.G + group_of(p, c));
+            if (BACKWARD) mu = (float)__ldg(p.mean + s_ * p.G + group_of(p, c)), rs = (float)__ldg(p.rstd + s_ * p.G + group_of(p, c));
         };
         if (c0 + (int)threadIdx.x < c1) known(c0 + threadIdx.x);
         if (second) {
             const Span v = p.spans[s_];
             const int windows = windows_of(p, v);
-            const Records r = records_of(p.of_window + first_window(p, v, s_) * p.G + g0, windows, p.offsets[s_], p.offsets[s_ + 1], (int64_t)v.b0 * p.rows, (int64_t)p.window * p.rows);
+            const Records<BACKWARD> r = records_of<BACKWARD>(p.of_window, first_window(p, v, s_) * p.G + g0, windows, p.offsets[s_], p.offsets[s_ + 1], (int64_t)v.b0 * p.rows, (int64_t)p.window * p.rows, p.W);
             if (!wait_for(sample_count(p) + s_, windows, p.status)) return false;
             merge_groups<BACKWARD>(p, r, group_of(p, c1 - 1) - g0 + 1, stats, scratch);
         }
@@ -356,12 +407,13 @@ struct Constants {
         for (int t = threadIdx.x; t < c1 - c0; t += NA_THREADS) {
             if (t >= NA_THREADS) known(c0 + t);
             const int col = t / VN, i = t % VN;
-            const float2 m = second ? stats[group_of(p, c0 + t) - g0] : make_float2(0.f, 0.f);
-            if (!BACKWARD) mu = m.x, rs = m.y;
+            Stats m = {};
+            if (second) m = stats[group_of(p, c0 + t) - g0];
+            if (!BACKWARD) mu = (float)m.x, rs = (float)m.y;
             float *to = at + ((i / QUAD) * l.cols + col) * QUAD + i % QUAD;
-            to[K_A * stride] = rs * w, to[K_B * stride] = BACKWARD ? bias : fmaf(-mu, rs * w, bias);
+            to[K_A * stride] = rs * w, to[K_B * stride] = BACKWARD ? bias : (float)fma(-(double)m.x, (double)m.y * w, (double)bias);
             if (BACKWARD) to[K_MU * stride] = -mu;
-            if (BACKWARD && second) to[K_M1 * stride] = -m.x * rs, to[K_M2 * stride] = -m.y * rs * rs;
+            if (BACKWARD && second) to[K_M1 * stride] = (float)-m.x * rs, to[K_M2 * stride] = (float)-m.y * rs * rs;
         }
         sync_workers();
         return true;
@@ -406,6 +458,12 @@ struct Rows {
     }
 };
 
+// What is taken off the values that are squared and summed: the first of them.  Values of 16 bits are multiples of a power of two, the
+// square of an odd multiple is 1 modulo 8, and so what does not fit a sum's 24 bits is rounded down nearly always: 4e-8 of the sum of squares,
+// however many rows.  A value a little beside theirs has no such pattern.  (Beside by 2^-11 of it: 16-bit values differ by more.)
+template <typename T>
+__device__ __forceinline__ float shift_of(float first) { return sizeof(T) == 4 ? first : first * 1.000457f; }
+
 template <typename T, int VN>
 __device__ __forceinline__ void stats_piece(const NormAct &p, const Columns &l, int64_t piece, int64_t lo, int n, float2 *fold) {
     constexpr int U = sizeof(T) == 4 && VN == 8 ? 2 : 4, P = (VN + 1) / 2;
@@ -424,7 +482,7 @@ __device__ __forceinline__ void stats_piece(const NormAct &p, const Columns &l, 
             in.load(col, r, n, l.lanes, p.C);
             float2 k[P];
 #pragma unroll
-            for (int j = 0; j < P; ++j) k[j] = neg2(pair_of(first, j));
+            for (int j = 0; j < P; ++j) k[j] = make_float2(-shift_of<T>(pair_of(first, j).x), -shift_of<T>(pair_of(first, j).y));
             for (; r < n; r += U * l.lanes) {
 #pragma unroll
                 for (int u = 0; u < U; ++u)
@@ -439,7 +497,7 @@ __device__ __forceinline__ void stats_piece(const NormAct &p, const Columns &l, 
         }
         fold_lanes<VN>(l, pass, a, b, fold, [&](int c, float sa, float sb) {
             const float off = sa / (float)n;
-            p.rec[piece * p.C + c] = make_float2(to_f32<T>(x[c]) + off, fmaxf(sb - sa * off, 0.f));
+            p.rec[piece * p.C + c] = make_float2(shift_of<T>(to_f32<T>(x[c])) + off, fmaxf(sb - sa * off, 0.f));
         });
     }
 }
@@ -452,8 +510,8 @@ __device__ __forceinline__ float2 drop2(const NormAct &p, const uint32_t *words,
 
 // ------------------------------------------------------------ second pass, forward ----
 template <typename T, int VN, int ACT, int DROP>
-__device__ __forceinline__ bool apply_piece(const NormAct &p, const Columns &l, const Philox<DROP != 1> &rng, Constants<VN> &k, int64_t s, int64_t lo, int n, bool owner) {
-    constexpr int U = (sizeof(T) == 4 && VN == 8 ? 2 : 4) / (DROP ? 2 : 1), P = (VN + 1) / 2, PAIRS = Constants<VN>::PAIRS;
+__device__ __forceinline__ bool apply_piece(const NormAct &p, const Columns &l, const Philox<DROP != 1> &rng, Constants<VN, false> &k, int64_t s, int64_t lo, int n, bool owner) {
+    constexpr int U = (sizeof(T) == 4 && VN == 8 ? 2 : 4) / (DROP ? 2 : 1), P = (VN + 1) / 2, PAIRS = Constants<VN, false>::PAIRS;
     const int64_t from = lo * p.C;
     const T *x = static_cast<const T *>(p.x) + from, *res = p.residual ? static_cast<const T *>(p.residual) + from : nullptr;
     T *y = static_cast<T *>(p.y) + from;
@@ -468,7 +526,7 @@ __device__ __forceinline__ bool apply_piece(const NormAct &p, const Columns &l, 
         if (res) q.load(res + c0, r, n, l.lanes, p.C);
         if (k.s != s || k.pass != pass) {
             sync_workers();
-            if (!k.template load<false>(p, l, s, pass, true)) return false;
+            if (!k.load(p, l, s, pass, true)) return false;
         }
         if (owner) k.put_stats(p, l);
         for (; r < n; r += U * l.lanes) {
@@ -478,7 +536,7 @@ __device__ __forceinline__ bool apply_piece(const NormAct &p, const Columns &l, 
                 for (int u = 0; u < U; ++u) rng.words<VN>((uint64_t)(from + (r + u * l.lanes) * p.C + c0), words[u]);
             }
 #pragma unroll
-            for (int h = 0; h < Constants<VN>::QUADS; ++h) {
+            for (int h = 0; h < Constants<VN, false>::QUADS; ++h) {
                 float2 a[PAIRS], b[PAIRS];
                 k.read(l, K_A, h, a), k.read(l, K_B, h, b);
 #pragma unroll
@@ -504,6 +562,17 @@ __device__ __forceinline__ bool apply_piece(const NormAct &p, const Columns &l, 
 }
 
 // ------------------------------------------------------------ backward ----
+// The ReLU's argument where 32 bits do not settle its sign: in fp64 it is the definition's.  That is asked for where the argument is this
+// small a part of what it is made of (its roundings are some 2^-23 of that), and for the sums alone: a sign that comes out on the
+// other side moves one element of the gradients of x and the residual, but a sum over a million rows by a whole gradient.
+constexpr float NEAR_BORDER = 0x1p-20f;
+__device__ __noinline__ float exact_argument(const NormAct &p, int64_t s, int c, float x, float residual) {
+    const int64_t g = s * p.G + group_of(p, c);
+    const double xh = ((double)x - __ldg(p.mean + g)) * __ldg(p.rstd + g);
+    return (float)((p.weight ? xh * __ldg(p.weight + c) + __ldg(p.bias + c) : xh) + residual);
+}
+enum { BORDER_AS_IT_IS = 0, BORDER_TOLD = 1, BORDER_SETTLED = 2 };
+
 // Rows of what both passes of the backward read, and gz of a pair of them.
 template <typename T, int VN, int ACT, int DROP, int U>
 struct BackwardRows {
@@ -522,20 +591,38 @@ struct BackwardRows {
             for (int u = 0; u < U; ++u) rng.words<VN>((uint64_t)(from + (r + u * l.lanes) * p.C), words[u]);
         }
     }
-    __device__ __forceinline__ float2 gz(const NormAct &p, int u, int j, float2 xc, float2 a, float2 b) const {
-        float2 z = fma2(xc, a, b);
-        if (p.residual) z = add2(z, pair_of(res.v[u], j));
-        const float2 v = act2_backward(ACT < 0 ? p.act : ACT, z, pair_of(g.v[u], j));
-        return (DROP < 0 ? p.drop.on : DROP) ? drop2<VN>(p, words[u], j, v) : v;
+    // x - mean and gz of COUNT pairs from the j0-th on, of sample s, the lump's first channel c0.  The answer: a ReLU's argument is next to
+    // its border (BORDER_TOLD).
+    template <int COUNT, int BORDER>
+    __device__ __forceinline__ bool gz(const NormAct &p, int64_t s, int c0, int u, int j0, const float2 *mu, const float2 *a, const float2 *b, float2 *xc, float2 *out) const {
+        const int act = ACT < 0 ? p.act : ACT;
+        bool near = false;
+#pragma unroll
+        for (int j = 0; j < COUNT; ++j) {
+            const float2 xs = pair_of(x.v[u], j0 + j), rs = p.residual ? pair_of(res.v[u], j0 + j) : both(0.f);
+            xc[j] = add2(xs, mu[j]);
+            float2 z = fma2(xc[j], a[j], b[j]);
+            if (p.residual) z = add2(z, rs);
+            if (BORDER != BORDER_AS_IT_IS && act == ACT_RELU) {
+                const float2 of = mul2(xs, a[j]);
+                const bool first = fabsf(z.x) < NEAR_BORDER * (fabsf(of.x) + fabsf(rs.x)), second = VN > 1 && fabsf(z.y) < NEAR_BORDER * (fabsf(of.y) + fabsf(rs.y));
+                near |= first | second;
+                if (BORDER == BORDER_SETTLED && first) z.x = exact_argument(p, s, c0 + 2 * (j0 + j), xs.x, rs.x);
+                if (BORDER == BORDER_SETTLED && second) z.y = exact_argument(p, s, c0 + 2 * (j0 + j) + 1, xs.y, rs.y);
+            }
+            const float2 v = act2_backward(act, z, pair_of(g.v[u], j0 + j));
+            out[j] = (DROP < 0 ? p.drop.on : DROP) ? drop2<VN>(p, words[u], j0 + j, v) : v;
+        }
+        return near;
     }
 };
 template <typename T, int VN>
 constexpr int BACKWARD_ROWS = sizeof(T) == 4 && VN == 8 ? 1 : 2;
 
 template <typename T, int VN, int ACT, int DROP>
-__device__ __forceinline__ void bwd_sums_piece(const NormAct &p, const Columns &l, const Philox<DROP != 1> &rng, Constants<VN> &k, int64_t piece, int64_t s, int64_t lo, int n,
+__device__ __forceinline__ void bwd_sums_piece(const NormAct &p, const Columns &l, const Philox<DROP != 1> &rng, Constants<VN, true> &k, int64_t piece, int64_t s, int64_t lo, int n,
                                                float2 *fold) {
-    constexpr int U = BACKWARD_ROWS<T, VN>, P = (VN + 1) / 2, PAIRS = Constants<VN>::PAIRS;
+    constexpr int U = BACKWARD_ROWS<T, VN>, P = (VN + 1) / 2, PAIRS = Constants<VN, true>::PAIRS;
     for (int pass = 0; pass < l.passes; ++pass) {
         const int lump = pass * l.cols + l.col;
         const int64_t from = lo * p.C + lump * VN;
@@ -547,35 +634,35 @@ __device__ __forceinline__ void bwd_sums_piece(const NormAct &p, const Columns &
         in.load(p, l, from, r, n);
         if (k.s != s || k.pass != pass) {
             sync_workers();
-            k.template load<true>(p, l, s, pass, false);
+            k.load(p, l, s, pass, false);
         }
         for (; r < n; r += U * l.lanes) {
             in.draw(p, l, rng, from, r);
 #pragma unroll
-            for (int h = 0; h < Constants<VN>::QUADS; ++h) {
+            for (int h = 0; h < Constants<VN, true>::QUADS; ++h) {
                 float2 mu[PAIRS], fa[PAIRS], fb[PAIRS];
                 k.read(l, K_MU, h, mu), k.read(l, K_A, h, fa), k.read(l, K_B, h, fb);
 #pragma unroll
                 for (int u = 0; u < U; ++u)
                     if (r + u * l.lanes < n)
+                    {
+                        float2 xc[PAIRS], gz[PAIRS];
+                        in.template gz<PAIRS, BORDER_SETTLED>(p, s, lump * VN, u, h * PAIRS, mu, fa, fb, xc, gz);
 #pragma unroll
-                        for (int i = 0; i < PAIRS; ++i) {
-                            const int j = h * PAIRS + i;
-                            const float2 xc = add2(pair_of(in.x.v[u], j), mu[i]), gz = in.gz(p, u, j, xc, fa[i], fb[i]);
-                            a[j] = add2(a[j], gz), b[j] = fma2(gz, xc, b[j]);
-                        }
+                        for (int i = 0; i < PAIRS; ++i) a[h * PAIRS + i] = add2(a[h * PAIRS + i], gz[i]), b[h * PAIRS + i] = fma2(gz[i], xc[i], b[h * PAIRS + i]);
+                    }
             }
             in.load(p, l, from, r + U * l.lanes, n);
         }
         fold_lanes<VN>(l, pass, a, b, fold, [&](int c, float sa, float sb) {
-            p.rec[piece * p.C + c] = make_float2(sa, sb * __ldg(p.rstd + s * p.G + group_of(p, c)));
+            p.rec[piece * p.C + c] = make_float2(sa, sb * (float)__ldg(p.rstd + s * p.G + group_of(p, c)));
         });
     }
 }
 
 template <typename T, int VN, int ACT, int DROP>
-__device__ __forceinline__ bool bwd_apply_piece(const NormAct &p, const Columns &l, const Philox<DROP != 1> &rng, Constants<VN> &k, int64_t s, int64_t lo, int n) {
-    constexpr int U = BACKWARD_ROWS<T, VN>, PAIRS = Constants<VN>::PAIRS;
+__device__ __forceinline__ bool bwd_apply_piece(const NormAct &p, const Columns &l, const Philox<DROP != 1> &rng, Constants<VN, true> &k, int64_t s, int64_t lo, int n) {
+    constexpr int U = BACKWARD_ROWS<T, VN>, PAIRS = Constants<VN, true>::PAIRS;
     T *dx = static_cast<T *>(p.dx), *dres = static_cast<T *>(p.dresidual);
     for (int pass = 0; pass < l.passes; ++pass) {
         const int lump = pass * l.cols + l.col;
@@ -585,23 +672,25 @@ __device__ __forceinline__ bool bwd_apply_piece(const NormAct &p, const Columns 
         in.load(p, l, from, r, n);   // (before the wait for the sums)
         if (k.s != s || k.pass != pass) {
             sync_workers();
-            if (!k.template load<true>(p, l, s, pass, true)) return false;
+            if (!k.load(p, l, s, pass, true)) return false;
         }
         for (; r < n; r += U * l.lanes) {
             in.draw(p, l, rng, from, r);
 #pragma unroll
-            for (int h = 0; h < Constants<VN>::QUADS; ++h) {
+            for (int h = 0; h < Constants<VN, true>::QUADS; ++h) {
                 float2 mu[PAIRS], fa[PAIRS], fb[PAIRS], m1[PAIRS], m2[PAIRS];
                 k.read(l, K_MU, h, mu), k.read(l, K_A, h, fa), k.read(l, K_B, h, fb), k.read(l, K_M1, h, m1), k.read(l, K_M2, h, m2);
 #pragma unroll
-                for (int u = 0; u < U; ++u)
+                for (int u = 0; u < U; ++u) {
+                    float2 xc[PAIRS], gz[PAIRS];
+                    in.template gz<PAIRS, BORDER_AS_IT_IS>(p, s, lump * VN, u, h * PAIRS, mu, fa, fb, xc, gz);
 #pragma unroll
                     for (int i = 0; i < PAIRS; ++i) {
                         const int j = h * PAIRS + i;
-                        const float2 xc = add2(pair_of(in.x.v[u], j), mu[i]), gz = in.gz(p, u, j, xc, fa[i], fb[i]);
-                        set_pair(in.g.v[u], j, gz);
-                        set_pair(in.x.v[u], j, fma2(gz, fa[i], fma2(xc, m2[i], m1[i])));
+                        set_pair(in.g.v[u], j, gz[i]);
+                        set_pair(in.x.v[u], j, fma2(gz[i], fa[i], fma2(xc[i], m2[i], m1[i])));
                     }
+                }
             }
 #pragma unroll
             for (int u = 0; u < U; ++u)
@@ -631,11 +720,11 @@ struct WarpTeam {
 
 // Merges the pieces of a window: a part of what merge_groups does, where records are many.
 template <bool BACKWARD, typename Team>
-__device__ __forceinline__ void merge_window(const NormAct &p, const Records &r, float2 *to) {
+__device__ __forceinline__ void merge_window(const NormAct &p, const Records<BACKWARD> &r, Record<BACKWARD> *to) {
     for (int g = Team::rank(); g < p.G; g += Team::SIZE) {
         RecordSums<BACKWARD> sums;
         sums.add(r, p.G, g, 0, 1);
-        to[g] = sums.done(r, (float)p.W);
+        to[g] = sums.done(r, p.W);
     }
 }
 
@@ -649,12 +738,13 @@ __device__ __forceinline__ int lanes_of_group(const NormAct &p) {
 
 // The records of a piece's groups, of `n` rows, from its channels' (`channel(c)`, visible to the team).
 template <bool BACKWARD, typename Team, typename Channel>
-__device__ __forceinline__ void group_records(const NormAct &p, int share, float inverse, int64_t piece, float n, Channel channel) {
+__device__ __forceinline__ void group_records(const NormAct &p, int share, int64_t piece, int n, Channel channel) {
     const int l = Team::rank() % share;
     const auto sum = [&](float v) {
         for (int o = share / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
         return v;
     };
+    Record<BACKWARD> *to = static_cast<Record<BACKWARD> *>(p.of_piece) + piece * p.G;
     for (int g0 = 0; g0 < p.G; g0 += Team::SIZE / share) {   // (the same rounds for all lanes of a warp)
         const int g = g0 + Team::rank() / share, c0 = min(g, p.G - 1) * p.W, end = g < p.G ? p.W : 0;
         float a = 0.f, b = 0.f;
@@ -666,19 +756,22 @@ __device__ __forceinline__ void group_records(const NormAct &p, int share, float
                 a += w * v.x, b += w * v.y;
             }
             a = sum(a), b = sum(b);
-        } else {   // the mean first, then squares about it
+            if (g < p.G && l == 0) to[g] = {a, b};
+        } else {   // the mean about the first channel's, then squares about it
             const float k = channel(c0).x;
 #pragma unroll 4
             for (int i = l; i < end; i += share) a += channel(c0 + i).x - k;
-            a = k + sum(a) * inverse;
+            const float off = sum(a) / (float)p.W;
 #pragma unroll 4
             for (int i = l; i < end; i += share) {
                 const float2 v = channel(c0 + i);
-                b += v.y + n * (v.x - a) * (v.x - a);
+                const float d = (v.x - k) - off;
+                b += v.y + (float)n * d * d;
             }
             b = sum(b);
+            const double mean = (double)k + off;
+            if (g < p.G && l == 0) to[g] = {(float)mean, (float)(mean - (double)(float)mean), b, 0.f};
         }
-        if (g < p.G && l == 0) p.of_piece[piece * p.G + g] = make_float2(a, b);
     }
 }
 
@@ -705,7 +798,8 @@ __device__ __forceinline__ void count_piece(const NormAct &p, const Span &v, int
         const int64_t number = first_window(p, v, s) + w, from = (int64_t)b * p.rows;
         if (!brings_the_last<Team>(window_count(p) + number, pieces, told)) return;
         const int64_t lo = max(p.offsets[s], from), hi = min(p.offsets[s + 1], from + (int64_t)pieces * p.rows);
-        merge_window<BACKWARD, Team>(p, records_of(p.of_piece + (b + s) * p.G, pieces, lo, hi, from, p.rows), p.of_window + number * p.G);
+        merge_window<BACKWARD, Team>(p, records_of<BACKWARD>(p.of_piece, (b + s) * p.G, pieces, lo, hi, from, p.rows, p.W),
+                                     static_cast<Record<BACKWARD> *>(p.of_window) + number * p.G);
     }
     Team::sync();
     if (Team::rank() == 0) {
@@ -742,7 +836,7 @@ template <int VN, bool BACKWARD>
 size_t shared_bytes(int C) {
     const Columns l(C, VN, 0);
     return (size_t)std::max(VN, 2) * NA_THREADS * sizeof(float2) + (size_t)(BACKWARD ? 8 : 3) * l.cols * VN * sizeof(float) +
-           (size_t)(2 * NA_THREADS + l.cols * VN + 2) * sizeof(float2);
+           NA_THREADS * sizeof(float4) + (size_t)(l.cols * VN + 1) * sizeof(Stats);
 }
 
 // ACT, DROP = -1: as the arguments say; DROP = 0: none, 1: the seed is in the arguments, 2: on the device.
@@ -753,10 +847,11 @@ __global__ void __launch_bounds__(NA_THREADS, BACKWARD ? 3 : 4) na_kernel(const 
     __shared__ int next, told;
     float2 *fold = reinterpret_cast<float2 *>(shared);   // sums of threads, or records that are merged
     const Columns l(p.C, VN, threadIdx.x);
-    Constants<VN> k_sums, k_apply;
+    Constants<VN, BACKWARD> k_sums, k_apply;
     k_apply.at = reinterpret_cast<float *>(fold + (VN < 2 ? 2 : VN) * NA_THREADS);
     k_sums.at = k_apply.at + 5 * l.cols * VN;
-    k_apply.scratch = reinterpret_cast<float4 *>(k_apply.at + ((BACKWARD ? 8 : 3) * l.cols * VN + 3) / 4 * 4), k_apply.stats = reinterpret_cast<float2 *>(k_apply.scratch + NA_THREADS);
+    k_apply.scratch = reinterpret_cast<float4 *>(k_apply.at + ((BACKWARD ? 8 : 3) * l.cols * VN + 3) / 4 * 4);
+    k_apply.stats = reinterpret_cast<Stats *>(k_apply.scratch + NA_THREADS);
     const Philox<DROP != 1> rng(p.drop);
     const int tiles = BACKWARD && p.dweight ? (p.C + AFFINE_CHANNELS - 1) / AFFINE_CHANNELS : 0;
     for (;;) {
@@ -781,7 +876,7 @@ __global__ void __launch_bounds__(NA_THREADS, BACKWARD ? 3 : 4) na_kernel(const 
                 else stats_piece<T, VN>(p, l, chunk + s, lo, (int)(hi - lo), fold);
                 sync_workers();
                 const float2 *channels = p.rec + (chunk + s) * p.C;   // (what this block has written)
-                group_records<BACKWARD, BlockTeam>(p, lanes_of_group<BlockTeam>(p), 1.f / (float)p.W, chunk + s, (float)(hi - lo), [&](int c) { return __ldcg(channels + c); });
+                group_records<BACKWARD, BlockTeam>(p, lanes_of_group<BlockTeam>(p), chunk + s, (int)(hi - lo), [&](int c) { return __ldcg(channels + c); });
                 count_piece<BACKWARD, BlockTeam>(p, p.spans[s], chunk, s, &told);
             } else {
                 bool there;
@@ -824,18 +919,19 @@ struct RingMemory {
     char *stages;
     float2 *fold;
     float *firsts, *constants;
-    float2 *stats, *scratch;
+    Stats *stats;
+    float4 *scratch;
     __device__ __forceinline__ RingMemory(const NormAct &p, char *shared) {
         stages = shared;
         fold = reinterpret_cast<float2 *>(shared + (size_t)p.stages * p.stage_bytes);
-        scratch = fold + FOLD_SLOTS * 8 * FOLD_STRIDE;
-        stats = scratch + 2 * NA_THREADS;   // (scratch: 256 sums of two doubles at most)
-        constants = reinterpret_cast<float *>(stats + p.C);
+        scratch = reinterpret_cast<float4 *>(fold + FOLD_SLOTS * 8 * FOLD_STRIDE);
+        stats = reinterpret_cast<Stats *>(scratch + NA_THREADS);
+        constants = reinterpret_cast<float *>(stats + p.G);
         firsts = constants + 3 * p.C;   // (forward alone)
     }
 };
-inline size_t ring_bytes(int C, bool backward) {   // without the tiles
-    return (size_t)(FOLD_SLOTS * 8 * FOLD_STRIDE + 2 * NA_THREADS + C) * sizeof(float2) + (size_t)(backward ? 8 : 3 + FOLD_SLOTS) * C * sizeof(float);
+inline size_t ring_bytes(int C, int G, bool backward) {   // without the tiles
+    return (size_t)FOLD_SLOTS * 8 * FOLD_STRIDE * sizeof(float2) + NA_THREADS * sizeof(float4) + (size_t)G * sizeof(Stats) + (size_t)(backward ? 8 : 3 + FOLD_SLOTS) * C * sizeof(float);
 }
 
 __device__ __forceinline__ void bulk_copy(uint32_t to, const void *from, uint32_t bytes, uint32_t bar, uint64_t policy) {
@@ -932,7 +1028,6 @@ __device__ __forceinline__ void ring_clerk(const NormAct &p, Ring &ring, const R
     const int lane = threadIdx.x & 31;
     const Columns l(p.C, 8, 0);
     const int lanes = warps_fold(l) ? NA_THREADS / 32 : l.lanes, share = lanes_of_group<WarpTeam>(p);
-    const float inverse = 1.f / (float)p.W;
     Place slot;
     for (;;) {
         slot.next(FOLD_SLOTS);
@@ -942,7 +1037,6 @@ __device__ __forceinline__ void ring_clerk(const NormAct &p, Ring &ring, const R
         float2 *fold = m.fold + slot.at * 8 * FOLD_STRIDE;
         const float *firsts = m.firsts + slot.at * p.C;
         const int64_t number = piece.chunk + (int64_t)piece.s;
-        const float each = 1.f / (float)piece.rows;
         for (int c = lane; c < p.C; c += 32) {
             float2 *from = fold + c % 8 * FOLD_STRIDE + c / 8;
             float a = 0.f, b = 0.f;
@@ -952,19 +1046,45 @@ __device__ __forceinline__ void ring_clerk(const NormAct &p, Ring &ring, const R
                 a += v.x, b += v.y;
             }
             if constexpr (BACKWARD) {
-                b *= __ldg(p.rstd + (int64_t)piece.s * p.G + group_of(p, c));
+                b *= (float)__ldg(p.rstd + (int64_t)piece.s * p.G + group_of(p, c));
                 if (p.dweight) p.rec[number * p.C + c] = make_float2(a, b);
             } else {
-                const float off = a * each;
+                const float off = a / (float)piece.rows;   // (not by a rounded inverse: its error is the same in every piece)
                 b = fmaxf(b - a * off, 0.f), a = firsts[c] + off;
             }
             *from = make_float2(a, b);
         }
         __syncwarp();
-        group_records<BACKWARD, WarpTeam>(p, share, inverse, number, (float)piece.rows, [&](int c) { return fold[c % 8 * FOLD_STRIDE + c / 8]; });
+        group_records<BACKWARD, WarpTeam>(p, share, number, piece.rows, [&](int c) { return fold[c % 8 * FOLD_STRIDE + c / 8]; });
         __syncwarp();
         if (lane == 0) tc::mbar_arrive(tc::smem_u32(&ring.taken[slot.at]));
         count_piece<BACKWARD, WarpTeam>(p, p.spans[piece.s], piece.chunk, piece.s, &ring.told);
+    }
+}
+
+// Sums of a thread, less what the lump at `from` gave them and more what it gives with its arguments' signs settled.
+struct TwoSums { float2 a[4], b[4]; };
+template <typename T, int DROP>
+__device__ __noinline__ void settle_sums(const NormAct &p, int64_t from, int64_t s, int c0, TwoSums *sums) {
+    BackwardRows<T, 8, ACT_RELU, DROP, 1> in;
+    in.x.v[0].load(static_cast<const T *>(p.x) + from), in.g.v[0].load(static_cast<const T *>(p.g) + from);
+    if (p.residual) in.res.v[0].load(static_cast<const T *>(p.residual) + from);
+    if (DROP) Philox<DROP != 1>(p.drop).template words<8>((uint64_t)from, in.words[0]);
+    float2 mu[4], a[4], b[4], xc[4], before[4], after[4];
+    for (int j = 0; j < 4; ++j) {
+        float v[6];
+        for (int i = 0; i < 2; ++i) {   // (as Constants::load makes them)
+            const int c = c0 + 2 * j + i;
+            const int64_t g = s * p.G + group_of(p, c);
+            v[i] = -(float)__ldg(p.mean + g), v[2 + i] = (float)__ldg(p.rstd + g) * (p.weight ? __ldg(p.weight + c) : 1.f), v[4 + i] = p.weight ? __ldg(p.bias + c) : 0.f;
+        }
+        mu[j] = make_float2(v[0], v[1]), a[j] = make_float2(v[2], v[3]), b[j] = make_float2(v[4], v[5]);
+    }
+    in.template gz<4, BORDER_AS_IT_IS>(p, s, c0, 0, 0, mu, a, b, xc, before);
+    in.template gz<4, BORDER_SETTLED>(p, s, c0, 0, 0, mu, a, b, xc, after);
+    for (int j = 0; j < 4; ++j) {
+        const float2 more = add2(after[j], neg2(before[j]));
+        sums->a[j] = add2(sums->a[j], more), sums->b[j] = fma2(more, xc[j], sums->b[j]);
     }
 }
 
@@ -978,9 +1098,9 @@ __device__ __forceinline__ void ring_worker(const NormAct &p, Ring &ring, const 
     const bool mine = l.lane < l.lanes;
     const int c0 = l.col * VN, step = l.lanes * p.C;   // elements from one of a thread's rows to its next
     const int tensor = p.tile_rows * p.C;              // elements from one tensor's tile to the next one's
-    Constants<8> k_sums, k_apply;
+    Constants<8, BACKWARD> k_sums, k_apply;
     k_apply.at = m.constants, k_sums.at = m.constants + 5 * p.C;
-    k_apply.stats = m.stats, k_apply.scratch = reinterpret_cast<float4 *>(m.scratch);
+    k_apply.stats = m.stats, k_apply.scratch = m.scratch;
     Place place, slot;
     int pieces = 0;
     Tile t;
@@ -1010,9 +1130,10 @@ __device__ __forceinline__ void ring_worker(const NormAct &p, Ring &ring, const 
             float2 a[P], b[P], k[P], fa[P], fb[P];   // k: what is taken off x
             const int s = t.s, chunk = t.chunk;
             int rows = 0;
+            int64_t unsettled = -1;   // a lump with a ReLU's argument next to its border (of two in a thread's part of a piece, the last)
             if (BACKWARD && k_sums.s != s) {
                 if (!sync_workers_and(true)) break;
-                k_sums.load<true>(p, l, s, 0, false);
+                k_sums.load(p, l, s, 0, false);
             }
             const bool free = next_slot();
 #pragma unroll
@@ -1023,10 +1144,10 @@ __device__ __forceinline__ void ring_worker(const NormAct &p, Ring &ring, const 
                 Lump<T, VN> v;
                 v.load(rows_at());
 #pragma unroll
-                for (int j = 0; j < P; ++j) k[j] = neg2(pair_of(v, j));
+                for (int j = 0; j < P; ++j) k[j] = make_float2(-shift_of<T>(pair_of(v, j).x), -shift_of<T>(pair_of(v, j).y));
                 if (l.lane == 0 && free) {
 #pragma unroll
-                    for (int q = 0; q < VN; ++q) m.firsts[slot.at * p.C + c0 + q] = v.get(q);
+                    for (int j = 0; j < P; ++j) *reinterpret_cast<float2 *>(m.firsts + slot.at * p.C + c0 + 2 * j) = neg2(k[j]);
                 }
             }
             for (bool more = true; more;) {
@@ -1039,16 +1160,18 @@ __device__ __forceinline__ void ring_worker(const NormAct &p, Ring &ring, const 
                         if constexpr (BACKWARD) {
                             in.g.v[0].load(x + tensor + at);
                             if (p.residual) in.res.v[0].load(x + 2 * tensor + at);
-                            if (DROP) rng.words<VN>((uint64_t)(t.from + at + c0), in.words[0]);
+                            if (DROP) rng.template words<VN>((uint64_t)(t.from + at + c0), in.words[0]);
                         }
+                        float2 xc[P], gz[P];
+                        if constexpr (BACKWARD)
+                            if (in.template gz<P, ACT == ACT_RELU ? BORDER_TOLD : BORDER_AS_IT_IS>(p, s, c0, 0, 0, k, fa, fb, xc, gz)) unsettled = t.from + at + c0;
 #pragma unroll
                         for (int j = 0; j < P; ++j) {
-                            const float2 xc = add2(pair_of(in.x.v[0], j), k[j]);
                             if constexpr (BACKWARD) {
-                                const float2 gz = in.gz(p, 0, j, xc, fa[j], fb[j]);
-                                a[j] = add2(a[j], gz), b[j] = fma2(gz, xc, b[j]);
+                                a[j] = add2(a[j], gz[j]), b[j] = fma2(gz[j], xc[j], b[j]);
                             } else {
-                                a[j] = add2(a[j], xc), b[j] = fma2(xc, xc, b[j]);
+                                xc[j] = add2(pair_of(in.x.v[0], j), k[j]);
+                                a[j] = add2(a[j], xc[j]), b[j] = fma2(xc[j], xc[j], b[j]);
                             }
                         }
                     }
@@ -1059,6 +1182,17 @@ __device__ __forceinline__ void ring_worker(const NormAct &p, Ring &ring, const 
                 if (t.kind == TILE_NONE) more = false;
             }
             if (!free) t.kind = TILE_NONE;
+            if constexpr (BACKWARD && ACT == ACT_RELU) {
+                if (unsettled >= 0) {
+                    TwoSums sums;
+#pragma unroll
+                    for (int j = 0; j < P; ++j) sums.a[j] = a[j], sums.b[j] = b[j];
+                    settle_sums<T, DROP>(p, unsettled, s, c0, &sums);
+#pragma unroll
+                    for (int j = 0; j < P; ++j) a[j] = sums.a[j], b[j] = sums.b[j];
+                }
+                __syncwarp();
+            }
             if (t.kind != TILE_NONE) {
                 if (warps_fold(l)) {   // over the warp's row lanes first
                     for (int o = 16; o >= l.cols; o >>= 1)
@@ -1079,7 +1213,7 @@ __device__ __forceinline__ void ring_worker(const NormAct &p, Ring &ring, const 
             const int s = t.s;
             if (k_apply.s != s) {
                 if (!sync_workers_and(true)) break;
-                if (!k_apply.load<BACKWARD>(p, l, s, 0, true)) break;
+                if (!k_apply.load(p, l, s, 0, true)) break;
             }
             float2 mu[P], fa[P], fb[P], m1[P], m2[P];
             k_apply.read_all(l, K_A, fa), k_apply.read_all(l, K_B, fb);
@@ -1095,13 +1229,14 @@ __device__ __forceinline__ void ring_worker(const NormAct &p, Ring &ring, const 
                         in.x.v[0].load(x + at);
                         if constexpr (BACKWARD) in.g.v[0].load(x + tensor + at);
                         if (p.residual) in.res.v[0].load(x + (BACKWARD ? 2 : 1) * tensor + at);
-                        if (DROP) rng.words<VN>((uint64_t)to, in.words[0]);
+                        if (DROP) rng.template words<VN>((uint64_t)to, in.words[0]);
+                        float2 xc[P], gz[P];
+                        if constexpr (BACKWARD) in.template gz<P, BORDER_AS_IT_IS>(p, s, c0, 0, 0, mu, fa, fb, xc, gz);
 #pragma unroll
                         for (int j = 0; j < P; ++j) {
                             if constexpr (BACKWARD) {
-                                const float2 xc = add2(pair_of(in.x.v[0], j), mu[j]), gz = in.gz(p, 0, j, xc, fa[j], fb[j]);
-                                set_pair(in.g.v[0], j, gz);
-                                set_pair(in.x.v[0], j, fma2(gz, fa[j], fma2(xc, m2[j], m1[j])));
+                                set_pair(in.g.v[0], j, gz[j]);
+                                set_pair(in.x.v[0], j, fma2(gz[j], fa[j], fma2(xc[j], m2[j], m1[j])));
                             } else {
                                 float2 z = fma2(pair_of(in.x.v[0], j), fa[j], fb[j]);
                                 if (p.residual) z = add2(z, pair_of(in.res.v[0], j));
@@ -1156,7 +1291,7 @@ int run_ring(const NormAct &p, cudaStream_t stream) {
     static std::atomic<uint64_t> allowed;
     if (int rc = allow_shared_memory((const void *)kernel, &allowed, true)) return rc;
     const int64_t tickets = 2 * (int64_t)p.chunks;
-    launch_after(kernel, (unsigned)std::min<int64_t>(tickets, RING_BLOCKS * num_sms()), RING_THREADS, (size_t)p.stages * p.stage_bytes + ring_bytes(p.C, BACKWARD), stream, p);
+    launch_after(kernel, (unsigned)std::min<int64_t>(tickets, RING_BLOCKS * num_sms()), RING_THREADS, (size_t)p.stages * p.stage_bytes + ring_bytes(p.C, p.G, BACKWARD), stream, p);
     PCX_LAUNCH_CHECK();
     return PCX_OK;
 }
