@@ -83,11 +83,20 @@ __global__ void __launch_bounds__(OFFSETS_THREADS) na_layout_kernel(const int64_
 }
 
 // ------------------------------------------------------------ host ----
-// Rows of a chunk: 32 KB of them, fewer where that would leave multiprocessors without one, whole rows of lanes.
+// Rows that are side by side in one of the ring's, as a power of two: as many as make whole lumps of eight channels, if that is no
+// row too long for it.
+int phase_bits_of(int C) {
+    int bits = 0;
+    while (((int64_t)C << bits) % 8) ++bits;
+    return ((int64_t)C << bits) <= RING_CHANNELS ? bits : 0;
+}
+
+// Rows of a chunk: 96 KB of them, fewer where that would leave multiprocessors without one, whole rows of lanes.
 int chunk_rows(int64_t N, int C, int dtype) {
+    const int bits = phase_bits_of(C);
     int vn = 8;
-    while (C % vn) vn /= 2;
-    const int lanes = Columns(C, vn, 0).lanes;
+    while ((C << bits) % vn) vn /= 2;
+    const int lanes = Columns(C << bits, vn, 0).lanes << bits;
     const int64_t by_bytes = NA_CHUNK_BYTES / ((int64_t)C * (int64_t)elem_size(dtype)), by_chip = (N + 4 * num_sms() - 1) / (4 * num_sms());
     return (int)std::max<int64_t>(1, (std::min(by_bytes, by_chip) + lanes - 1) / lanes) * lanes;
 }
@@ -117,20 +126,22 @@ bool sizes_ok(int64_t N, int64_t S, int C, int G, int dtype, int activation) {
 
 // Both launches of a direction.
 template <bool BACKWARD>
-int run(const int64_t *d_lengths, NormAct &p, int dtype, int vn, int activation, cudaStream_t stream) {
+int run(const int64_t *d_lengths, NormAct &p, int dtype, int activation, std::initializer_list<const void *> tensors_at, cudaStream_t stream) {
+    const int vn = lump_of(p.C, dtype, tensors_at);
     p.act = activation;
     if (int rc = device_status_address(&p.status)) return rc;
     const int64_t lag = NA_LAG_BYTES / ((int64_t)p.rows * p.C * (int64_t)elem_size(dtype) * (BACKWARD ? 2 : 1));
     p.lag = (int)std::max<int64_t>(1, std::min<int64_t>(lag, p.chunks));
-    p.stages = 0;
-    if (vn == 8 && p.C <= RING_CHANNELS) {   // the ring
-        const int lanes = Columns(p.C, 8, 0).lanes, tensors = (BACKWARD ? 2 : 1) + (p.residual ? 1 : 0), row_bytes = p.C * (int)elem_size(dtype);
+    p.stages = 0, p.phase_bits = phase_bits_of(p.C), p.V = p.C << p.phase_bits;
+    if (lump_of(p.V, dtype, tensors_at) == 8 && p.V <= RING_CHANNELS) {   // the ring
+        const int lanes = Columns(p.V, 8, 0).lanes, tensors = (BACKWARD ? 2 : 1) + (p.residual ? 1 : 0), row_bytes = p.V * (int)elem_size(dtype);
         p.tile_rows = lanes * std::max(1, NA_STAGE_BYTES / (lanes * row_bytes * tensors));
         p.sums_tile_rows = BACKWARD ? p.tile_rows : p.tile_rows * tensors;
         p.stage_bytes = (p.tile_rows * row_bytes * tensors + 127) / 128 * 128;
-        p.stages = std::min(RING_STAGES, (NA_RING_BYTES - (int)ring_bytes(p.C, p.G, BACKWARD)) / p.stage_bytes);
+        p.stages = std::min(RING_STAGES, (NA_RING_BYTES - (int)ring_bytes(p.V, p.G, BACKWARD)) / p.stage_bytes);
         if (p.stages < 2) p.stages = 0;
     }
+    if (!p.stages) p.phase_bits = 0;
     launch_after(na_layout_kernel<BACKWARD>, 1, p.S <= 256 ? 256 : OFFSETS_THREADS, 0, stream, d_lengths, p);
     PCX_LAUNCH_CHECK();
     if (p.N == 0) {
@@ -178,9 +189,8 @@ int pcx_ragged_group_norm_act(const void *d_x, const int64_t *d_lengths, const f
     if (ws_bytes < need) PCX_FAIL(PCX_E_CAPACITY, "pcx_ragged_group_norm_act: workspace %zu < %zu bytes", ws_bytes, need);
     p.x = d_x, p.residual = d_residual, p.y = d_y, p.weight = d_weight, p.bias = d_bias, p.mean = d_mean, p.rstd = d_rstd;
     p.N = N, p.S = S, p.C = C, p.G = G, p.W = C / G, p.by_width = (uint32_t)((0xFFFFFFFFull + p.W) / p.W), p.eps = eps;
-    const int vn = lump_of(C, dtype, {d_x, d_residual, d_y});
     prof_begin("group_norm_act(fwd)", stream);
-    const int rc = run<false>(d_lengths, p, dtype, vn, activation, stream);
+    const int rc = run<false>(d_lengths, p, dtype, activation, {d_x, d_residual, d_y}, stream);
     prof_end(stream);
     return rc;
 }
@@ -204,9 +214,8 @@ int pcx_ragged_group_norm_act_backward(const void *d_grad_y, const void *d_x, co
     p.x = d_x, p.residual = d_residual, p.g = d_grad_y, p.dx = d_grad_x, p.dresidual = d_grad_residual, p.weight = d_weight, p.bias = d_bias;
     p.mean = const_cast<double *>(d_mean), p.rstd = const_cast<double *>(d_rstd), p.dweight = d_grad_weight, p.dbias = d_grad_bias;
     p.N = N, p.S = S, p.C = C, p.G = G, p.W = C / G, p.by_width = (uint32_t)((0xFFFFFFFFull + p.W) / p.W);
-    const int vn = lump_of(C, dtype, {d_x, d_residual, d_grad_y, d_grad_x, d_grad_residual});
     prof_begin("group_norm_act(bwd)", stream);
-    const int rc = run<true>(d_lengths, p, dtype, vn, activation, stream);
+    const int rc = run<true>(d_lengths, p, dtype, activation, {d_x, d_residual, d_grad_y, d_grad_x, d_grad_residual}, stream);
     prof_end(stream);
     return rc;
 }

@@ -112,6 +112,12 @@ struct Lump {
 #pragma unroll
         for (int q = 0; q < BYTES / 16; ++q) __stcs(reinterpret_cast<uint4 *>(p) + q, make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]));
     }
+    // The elements first <= i < end.
+    __device__ __forceinline__ void store_part(T *__restrict__ p, int first, int end) const {
+#pragma unroll
+        for (int i = 0; i < VN; ++i)
+            if (i >= first && i < end) p[i] = reinterpret_cast<const T *>(w)[i];
+    }
     __device__ __forceinline__ float get(int i) const { return to_f32<T>(reinterpret_cast<const T *>(w)[i]); }
     __device__ __forceinline__ void set(int i, float v) { reinterpret_cast<T *>(w)[i] = from_f32<T>(v); }
 };

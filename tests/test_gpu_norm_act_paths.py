@@ -1,0 +1,144 @@
+"""``fused_group_norm_act`` where its kernels take other ways: rows that are no multiple of 16 bytes, samples that end inside of one, the
+widths up to which rows are brought by bulk copies, many groups in many pieces, several streams and graphs at a time."""
+import ctypes
+import os
+import subprocess
+import sys
+
+import pytest
+import torch
+
+from test_gpu_norm_act import DEV, RNG, _check, _make, _run
+
+pytestmark = pytest.mark.gpu
+
+# samples begin and end at every row of 2, 4 and 8 that lie side by side; one is several pieces long
+RAGGED = [1, 1, 2, 3, 0, 5, 7, 1, 11, 2003, 0, 1, 4, 9]
+
+
+@pytest.mark.parametrize("C", [1, 3, 6, 7, 12, 33, 50, 100, 126, 127, 129, 130, 254, 258, 500, 516])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("act,p,residual", [("relu", 0.0, True), ("gelu", 0.3, False)])
+def test_rows_side_by_side(C, dtype, act, p, residual):
+    """Twice the width: 2 to 8 rows are a row of the ring, up to 1024 channels (127 and 129, 254 and 258, 500 and 516 are about the limit)."""
+    groups = next(g for g in (5, 4, 3, 2, 1) if C % g == 0)
+    _check(_make(RAGGED, C, dtype, C), RAGGED, groups, act, p, residual=residual)
+
+
+@pytest.mark.parametrize("N", range(1, 18))
+@pytest.mark.parametrize("C", [1, 5, 6])
+def test_ends_of_a_tensor(N, C):
+    """The last bytes are no multiple of 16; there may be nothing else."""
+    for dtype in (torch.float32, torch.bfloat16):
+        _check(_make([N], C, dtype, N), [N], 1, "silu")
+
+
+@pytest.mark.parametrize("C", [33, 50, 100])
+def test_neighbours_do_not_meet(C):
+    """A sample of NaN and infinities between two others that share 16 bytes with it."""
+    lengths = [37, 3, 201]
+    t = _make(lengths, C, torch.bfloat16, C)
+    y, grads = _run(t, lengths, 1, "relu")
+    bad = {k: v.clone() for k, v in t.items()}
+    bad["x"][37:40] = torch.tensor([float("nan"), float("inf"), -float("inf")], device=DEV).bfloat16()[:, None]
+    bad["grad"][37:40] = float("nan")
+    yb, gb = _run(bad, lengths, 1, "relu")
+    for a, b in ((y, yb), (grads["x"], gb["x"]), (grads["residual"], gb["residual"])):
+        assert torch.equal(a[:37], b[:37]) and torch.equal(a[40:], b[40:])
+    assert gb["x"][37:40].isnan().all()
+
+
+@pytest.mark.parametrize("C", [33, 50, 64])
+def test_nothing_is_written_behind_the_tensors(C):
+    from pointelligence_b200 import _cabi
+
+    h, N, S, G, extra = _cabi.lib(), 1003, 3, 1, 64
+    lengths = torch.tensor([500, 2, 501], device=DEV)
+    for dtype in (torch.float32, torch.bfloat16):
+        code = _cabi._DTYPES[dtype]
+        x, g = torch.randn(N, C, device=DEV).to(dtype), torch.randn(N, C, device=DEV).to(dtype)
+        y, dx, dres = (torch.full((N * C + extra,), 7.0, dtype=dtype, device=DEV) for _ in range(3))
+        mean, rstd = (torch.full((S * G + extra,), 7.0, dtype=torch.double, device=DEV) for _ in range(2))
+        ws = torch.empty(h.pcx_ragged_group_norm_act_workspace_bytes(N, S, C, G, code), dtype=torch.uint8, device=DEV)
+        P, stream = _cabi.ptr, ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+        _cabi.check(h.pcx_ragged_group_norm_act(P(x), P(lengths), None, None, None, P(y), P(mean), P(rstd), N, S, C, G, 1e-5, 2, 0.0, 0, 0, None, code, P(ws), ws.numel(), stream))
+        _cabi.check(h.pcx_ragged_group_norm_act_backward(P(g), P(x), None, P(lengths), None, None, P(mean), P(rstd), P(dx), None, None, P(dres), N, S, C, G, 2, 0.0, 0, 0, None, code,
+                                                         P(ws), ws.numel(), stream))
+        torch.cuda.synchronize()
+        for t in (y, dx, dres, mean, rstd):
+            assert bool((t[-extra:] == 7).all()) and bool((t[:-extra] != 7).any())
+
+
+@pytest.mark.parametrize("C", [1016, 1024, 1032, 2048])
+def test_widest_rows(C):
+    lengths = [700, 0, 44]
+    _check(_make(lengths, C, torch.float16, C), lengths, 4, "relu", 0.3)
+
+
+@pytest.mark.parametrize("C,groups,lengths", [(256, 256, [5000]), (256, 256, [2500, 1, 0, 3000]), (250, 250, [4000, 900]), (1032, 1032, [900, 33]), (64, 64, [30000, 20000, 5])])
+def test_many_groups_in_many_pieces(C, groups, lengths):
+    """So many records that they are merged in windows first."""
+    _check(_make(lengths, C, torch.bfloat16, C), lengths, groups, "silu")
+
+
+def test_several_streams_at_a_time():
+    """Calls of two streams that run side by side, and graphs of one memory pool replayed in turn, answer as calls alone do."""
+    cases = [(_make([40000, 2000], 64, torch.bfloat16, 1), [40000, 2000], 8), (_make([30000, 1, 5000], 50, torch.bfloat16, 2), [30000, 1, 5000], 5)]
+    alone = [_run(t, lengths, groups, "silu", 0.1) for t, lengths, groups in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    for _ in range(5):
+        got = []
+        for stream, (t, lengths, groups) in zip(streams, cases):
+            with torch.cuda.stream(stream):
+                got.append(_run(t, lengths, groups, "silu", 0.1))
+        torch.cuda.synchronize()
+        for (y, grads), (y1, grads1) in zip(alone, got):
+            assert torch.equal(y, y1) and all(torch.equal(grads[k], grads1[k]) for k in grads)
+    from pointelligence_b200.layers.norm import fused_group_norm_act
+
+    with torch.no_grad():
+        lens = [torch.tensor(lengths, device=DEV) for _, lengths, _ in cases]
+        step = lambda k: fused_group_norm_act(cases[k][0]["x"], lens[k], cases[k][2], cases[k][0]["weight"], cases[k][0]["bias"], residual=cases[k][0]["residual"],
+                                              activation="silu", dropout=0.1, rng=RNG)
+        graphs, outs = [torch.cuda.CUDAGraph() for _ in cases], []
+        pool = torch.cuda.graph_pool_handle()
+        for k, graph in enumerate(graphs):
+            with torch.cuda.graph(graph, pool=pool):
+                outs.append(step(k))
+        for _ in range(4):
+            for k, graph in enumerate(graphs):
+                graph.replay()
+                torch.cuda.synchronize()
+                assert torch.equal(outs[k], alone[k][0])
+
+
+PART_OF_THE_CHIP = """
+import torch
+from pointelligence_b200.layers.norm import fused_group_norm_act
+torch.zeros(1, device="cuda")
+part = torch.cuda.GreenContext.create(16, 0)
+stream = part.Stream()
+for C, groups in ((64, 8), (50, 5), (1032, 4), (64, 64)):
+    g = torch.Generator(device="cuda").manual_seed(C)
+    x = (torch.randn(20000, C, device="cuda", generator=g) * 2 + 3).bfloat16().requires_grad_()
+    go = torch.randn(20000, C, device="cuda", generator=g).bfloat16()
+    w, b = torch.ones(C, device="cuda").requires_grad_(), torch.zeros(C, device="cuda").requires_grad_()
+    lengths = torch.tensor([15000, 5000], device="cuda")
+    step = lambda: torch.autograd.grad(fused_group_norm_act(x, lengths, groups, w, b, activation="silu", dropout=0.2, rng=(1, 8)), (x, w, b), go)
+    whole = step()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        got = step()
+    stream.synchronize()
+    assert all(torch.equal(a, r) for a, r in zip(got, whole)), C
+"""
+
+
+def test_on_a_part_of_the_chip():
+    """A stream that has fewer multiprocessors than the blocks of one launch would take together."""
+    if not hasattr(torch.cuda, "GreenContext"):
+        pytest.skip("no green contexts")
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    done = subprocess.run([sys.executable, "-c", PART_OF_THE_CHIP], cwd=root, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stderr[-2000:]
