@@ -4,8 +4,9 @@
 //
 // A unit u is an element (row-major index), a channel of a sample (s * C + c: feature dropout) or a sample (s: drop path, which
 // drops a residual branch whole).  Backward, with g masked where y > 0 does not hold (relu): dresidual = g, dx = keep[u] * g / (1 - p).
-// What is dropped is zero whatever it was, and rows of a dropped sample are not read.  Bound by bytes; by element a generator
-// call makes the words of eight elements, 7.5 operations each, beside the memory's work.
+// What is dropped is zero whatever it was, and rows of a dropped sample are not read.  Bound by bytes: by element, 730 thousand rows of 96
+// channels, bf16, 280 MB in 46 us, 6.1 TB/s (a copy's 6.5), beside which a generator call for every eight elements has room; by
+// sample with residual and ReLU, 500 thousand rows of 64 channels, p = 0.3, 173 MB in 32 us forward and 256 MB in 42 us backward.
 #include <algorithm>
 
 #include "philox.cuh"

@@ -630,6 +630,7 @@ py::object draw_rng_for(const Tensor &like) {
 
 void require_rows(const Tensor &x) {
     require(x.dim() == 2, PyExc_ValueError, [&] { return "expected rows (points, channels), got " + str(x.sizes()); });
+    require(x.size(1) <= INT32_MAX, PyExc_ValueError, [] { return std::string("rows have at most 2^31 - 1 channels"); });
 }
 void require_like(const char *name, const OptTensor &t, const Tensor &x, at::IntArrayRef sizes) {
     if (!t) return;

@@ -54,7 +54,7 @@ class RaggedDropout(nn.Module):
     def forward(self, x, lengths=None, residual=None, relu=False, rng=None):
         if self.training and self.p > 0.0:
             return fused_dropout(x, self.p, rng, self.unit, lengths, residual, relu)
-        x = x if residual is None else x + residual
+        x = x if residual is None else x + residual.to(x.dtype)
         return x.relu() if relu else x
 
     def extra_repr(self):

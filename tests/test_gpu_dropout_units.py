@@ -36,3 +36,12 @@ def test_neighbours_and_rows_not_read(unit, C):
     assert 0.3 < dropped.float().mean() < 0.7
     bad = torch.where(dropped, torch.full_like(x, float("nan")), x)
     assert torch.equal(fused_dropout(bad, 0.5, rng=RNG, unit=unit, lengths=lengths), y)
+
+
+def test_rows_too_long():
+    from pointelligence_b200.layers.dropout import fused_dropout
+
+    x = torch.zeros(1, dtype=torch.float16, device=DEV).expand(4, 2 ** 32 + 8)
+    for unit in ("channel", "sample"):
+        with pytest.raises(ValueError, match="channels"):
+            fused_dropout(x, 0.5, unit=unit, lengths=torch.tensor([4], device=DEV))

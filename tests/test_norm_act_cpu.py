@@ -134,3 +134,15 @@ def test_network_arguments():
     for bad in (dict(activation="tanh"), dict(dropout=1.5), dict(drop_path=-0.1), dict(norm_groups=7)):
         with pytest.raises(ValueError):
             ResUNet(**bad)
+
+
+def test_rows_too_long():
+    x = torch.zeros(1, dtype=torch.float16).expand(4, 2 ** 32 + 8)
+    with pytest.raises(ValueError, match="channels"):
+        fused_group_norm_act(x, LENGTHS, 2)
+
+
+def test_the_layer_keeps_its_type_without_training():
+    layer = RaggedDropout(0.5).eval()
+    y = layer(torch.ones(2, 3, dtype=torch.bfloat16), residual=torch.full((2, 3), 0.25), relu=True)
+    assert y.dtype == torch.bfloat16 and bool((y == 1.25).all())
