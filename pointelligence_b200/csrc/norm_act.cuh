@@ -1091,9 +1091,11 @@ template <bool BACKWARD, bool PHASES>
 __device__ __forceinline__ void ring_clerk(const NormAct &p, Ring &ring, const RingMemory &m) {
     const int lane = threadIdx.x & 31;
     const Columns l(p.V, 8, 0);
-    int parts = 1;   // lanes of a channel
-    while (2 * parts * p.C <= 32) parts *= 2;
-    const int lanes = warps_fold(l) ? NA_THREADS / 32 : l.lanes, share = lanes_of_group<WarpTeam>(p);
+    const int lanes = warps_fold(l) ? NA_THREADS / 32 : l.lanes;
+    const bool few = !PHASES && lanes <= 8;   // one chain (with eight, a call of 942 points and 256 channels takes a microsecond more)
+    int parts = 1;                            // lanes of a channel
+    while (!few && 2 * parts * p.C <= 32) parts *= 2;
+    const int share = lanes_of_group<WarpTeam>(p);
     Place slot;
     for (;;) {
         slot.next(FOLD_SLOTS);
@@ -1105,10 +1107,19 @@ __device__ __forceinline__ void ring_clerk(const NormAct &p, Ring &ring, const R
         const int64_t number = piece.chunk + (int64_t)piece.s;
         for (int base = 0; base < p.C; base += 32 / parts) {   // (the same rounds for all lanes)
             const int c = base + lane / parts;
-            Chains chains;
-            if (c < p.C)
-                for (int at = c; at < (PHASES ? p.V : c + 1); at += p.C) chains.add(fold + at % 8 * FOLD_STRIDE + at / 8, lane % parts, parts, lanes, l.cols);
-            float2 sums = chains.sum();
+            float2 sums = make_float2(0.f, 0.f);
+            if (few) {
+                if (c >= p.C) continue;
+                const float2 *from = fold + c % 8 * FOLD_STRIDE + c / 8;
+#pragma unroll
+                for (int q = 0; q < 8; ++q)
+                    if (q < lanes) sums = add2(sums, from[q * l.cols]);
+            } else {
+                Chains chains;
+                if (c < p.C)
+                    for (int at = c; at < (PHASES ? p.V : c + 1); at += p.C) chains.add(fold + at % 8 * FOLD_STRIDE + at / 8, lane % parts, parts, lanes, l.cols);
+                sums = chains.sum();
+            }
             for (int o = parts / 2; o > 0; o >>= 1) sums = add2(sums, make_float2(__shfl_xor_sync(0xffffffffu, sums.x, o), __shfl_xor_sync(0xffffffffu, sums.y, o)));
             if (c >= p.C || lane % parts) continue;
             float a = sums.x, b = sums.y;

@@ -142,3 +142,27 @@ def test_on_a_part_of_the_chip():
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     done = subprocess.run([sys.executable, "-c", PART_OF_THE_CHIP], cwd=root, capture_output=True, text=True, timeout=300)
     assert done.returncode == 0, done.stderr[-2000:]
+
+
+def test_rows_side_by_side_past_32_bits():
+    """More than 2^32 elements in rows of 50: the last sample of a long batch is what it is alone."""
+    from pointelligence_b200.layers.norm import fused_group_norm_act
+
+    C, tail = 50, 3001
+    N = 2 ** 32 // C + tail
+    g = torch.Generator(device=DEV).manual_seed(0)
+    x = torch.empty(N, C, dtype=torch.bfloat16, device=DEV)
+    x.normal_(generator=g)
+    w, b = torch.randn(C, device=DEV, generator=g), torch.randn(C, device=DEV, generator=g)
+    go = torch.zeros_like(x)
+    go[-tail:].normal_(generator=g)
+    x.requires_grad_()
+    y = fused_group_norm_act(x, torch.tensor([N - tail - 5, 5, tail], device=DEV), 5, w, b)
+    dx, = torch.autograd.grad(y, x, go)
+    alone = x.detach()[-tail:].clone().requires_grad_()
+    y1 = fused_group_norm_act(alone, torch.tensor([tail], device=DEV), 5, w, b)
+    dx1, = torch.autograd.grad(y1, alone, go[-tail:])
+    # pieces are cut at other rows: statistics differ by roundings of 32 bits, results by one of 16
+    assert float((y.detach()[-tail:].double() - y1.detach().double()).norm() / y1.detach().double().norm()) < 2.0 ** -9
+    assert float((dx[-tail:].double() - dx1.double()).norm() / dx1.double().norm()) < 2.0 ** -9
+    assert not dx[:-tail].any()
