@@ -1,5 +1,7 @@
 // Entry points of the group norm with activation and dropout (norm_act.cuh): arguments, workspace, and the launch that lays the
 // samples out.
+#include <cmath>
+
 #include "norm_act.cuh"
 
 namespace pcx {
@@ -15,7 +17,7 @@ constexpr int NA_CHUNK_BYTES = 96 << 10;        // of x
 constexpr int NA_STAGE_BYTES = 24 << 10;        // of a tile, all tensors
 constexpr int NA_RING_BYTES = 110 << 10;        // of shared memory, a block: two on a multiprocessor
 constexpr int NA_MAX_C = 1 << 16;
-constexpr int NA_RECORDS = 8 << 10;             // of groups that a block reads for itself, at most: 128 KB where all rows are one sample's
+constexpr int NA_RECORDS = 8 << 10;             // of groups that a block reads for itself without windows: 128 KB where all rows are one sample's
 constexpr int64_t NA_LAG_BYTES = 64 << 20;      // of x, and of the gradient
 
 // ------------------------------------------------------------ the samples' rows ----
@@ -101,6 +103,16 @@ int chunk_rows(int64_t N, int C, int dtype) {
     return (int)std::max<int64_t>(1, (std::min(by_bytes, by_chip) + lanes - 1) / lanes) * lanes;
 }
 
+// Pieces of a window: as many as leave a block NA_RECORDS records to read for itself, but not so many that the warp that merges a
+// window takes longer than all blocks with theirs: that time grows with the window, the blocks' with the number of windows, and at 1458
+// pieces they are alike at eight (one sample of 273 thousand rows, 256 instance norms, bf16, forward: windows of 4, 8, 16 and 46 (as
+// NA_RECORDS alone has it) pieces 187, 181, 203 and 278 us).
+int window_of(int chunks, int G) {
+    const int64_t by_records = (chunks * (int64_t)G + NA_RECORDS - 1) / NA_RECORDS;
+    const int64_t by_turns = std::max<int64_t>(8, (int64_t)std::sqrt(chunks / 24.0));
+    return (int)std::max<int64_t>(1, std::min(by_records, by_turns));
+}
+
 size_t carve(void *ws, int64_t N, int64_t S, int C, int G, int dtype, NormAct *out) {
     Carver c(ws);
     NormAct p = out ? *out : NormAct{};
@@ -109,7 +121,7 @@ size_t carve(void *ws, int64_t N, int64_t S, int C, int G, int dtype, NormAct *o
     p.offsets = c.take<int64_t>((size_t)S + 1);
     p.spans = c.take<Span>((size_t)S);
     p.rec = c.take<float2>((size_t)(p.chunks + S) * C);
-    p.window = (int)std::max<int64_t>(1, (p.chunks * (int64_t)G + NA_RECORDS - 1) / NA_RECORDS);
+    p.window = window_of(p.chunks, G);
     const size_t windows = p.window > 1 ? (size_t)windows_in_all(p.chunks, S, p.window) : 0;
     p.of_piece = c.take<float4>((size_t)(p.chunks + S) * G);   // (backward: of float2)
     p.of_window = windows ? c.take<float4>(windows * G) : p.of_piece;
