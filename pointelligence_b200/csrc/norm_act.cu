@@ -93,14 +93,18 @@ int phase_bits_of(int C) {
     return ((int64_t)C << bits) <= RING_CHANNELS ? bits : 0;
 }
 
-// Rows of a chunk: 96 KB of them, fewer where that would leave multiprocessors without one, whole rows of lanes.
+// Rows of a chunk: 96 KB of them at most, and as many as give every block of the chip the same number of chunks, in whole rows of lanes.
+// (With two for a block wherever they were small, some blocks had two and some one: 20 thousand rows of 50 channels, fp32, 30 us
+// forward and 34 backward for 20 and 24, 5000 of 256, fp16, with dropout 28 and 32 for 22 and 28; with one, whatever 96 KB allow, 200
+// thousand of 96, bf16, 40 for 35.)
 int chunk_rows(int64_t N, int C, int dtype) {
     const int bits = phase_bits_of(C);
     int vn = 8;
     while ((C << bits) % vn) vn /= 2;
     const int lanes = Columns(C << bits, vn, 0).lanes << bits;
-    const int64_t by_bytes = NA_CHUNK_BYTES / ((int64_t)C * (int64_t)elem_size(dtype)), by_chip = (N + 4 * num_sms() - 1) / (4 * num_sms());
-    return (int)std::max<int64_t>(1, (std::min(by_bytes, by_chip) + lanes - 1) / lanes) * lanes;
+    const int64_t most = std::max<int64_t>(1, NA_CHUNK_BYTES / ((int64_t)C * (int64_t)elem_size(dtype))), blocks = RING_BLOCKS * num_sms();
+    const int64_t rounds = std::max<int64_t>(1, (N + most * blocks - 1) / (most * blocks)), rows = (N + rounds * blocks - 1) / (rounds * blocks);
+    return (int)((std::max<int64_t>(rows, 1) + lanes - 1) / lanes) * lanes;
 }
 
 // Pieces of a window: as many as leave a block NA_RECORDS records to read for itself, but not so many that the warp that merges a

@@ -929,10 +929,10 @@ __global__ void __launch_bounds__(NA_THREADS, BACKWARD ? 3 : 4) na_kernel(const 
 //
 // Bound by bytes where the tail is short, every input read once a pass: 1.1 million points of 64 channels, bf16, eight samples, ReLU and
 // residual: forward 563 MB in 106 us, 5.3 TB/s; backward 1126 MB in 222 us, 5.1 TB/s, where 6.5 TB/s are a copy's.  By instructions with
-// SiLU and dropout of 0.1: 422 MB in 126 us, 704 MB in 225 us (without dropout 105 and 195).  Where all rows are some megabytes the
-// launch is latency: one sample of 942 points and 256 channels 12 us, of which a first read, the records' turn through the L2 and the
-// code's own way into the instruction cache are most.  (A second read of x from the L2 was aimed at, with a lag of few chunks: what is in
-// flight at a time, some 70 MB with the gradient, is more than the L2 keeps beside what is written, and shorter lags wait for records.)
+// SiLU and dropout of 0.1: 422 MB in 125 us, 704 MB in 225 us (without dropout 99 and 177).  Where all rows are some megabytes the
+// launch is latency: one sample of 942 points and 256 channels 12 to 15 us, of which a first read, the records' turn through the L2 and the
+// code's own way into the instruction cache are most.  (Lags of few chunks, so that the second pass finds its rows in the L2, do not pay:
+// what is in flight until a sample's records are there is as much as the L2 keeps beside what is written.)
 enum { TILE_SUMS = 0, TILE_APPLY = 1, TILE_AFFINE = 2, TILE_END = 3, TILE_NONE = 4 };
 constexpr int RING_CHANNELS = 1024;                // of a row, at most (their constants take room from the ring)
 constexpr int RING_STAGES = 8;                     // at most
