@@ -151,10 +151,14 @@ int run(const int64_t *d_lengths, NormAct &p, int dtype, int activation, std::in
     p.stages = 0, p.phase_bits = phase_bits_of(p.C), p.V = p.C << p.phase_bits;
     if (lump_of(p.V, dtype, tensors_at) == 8 && p.V <= RING_CHANNELS) {   // the ring
         const int lanes = Columns(p.V, 8, 0).lanes, tensors = (BACKWARD ? 2 : 1) + (p.residual ? 1 : 0), row_bytes = p.V * (int)elem_size(dtype);
-        p.tile_rows = lanes * std::max(1, NA_STAGE_BYTES / (lanes * row_bytes * tensors));
+        const int room = NA_RING_BYTES - (int)ring_bytes(p.V, p.G, BACKWARD);
+        // (Where two tiles of 24 KB do not fit, smaller ones: 1024 channels, bf16, backward 292 us of 70 million elements, 458 by the general
+        // kernel; where they do, three of two thirds are no better: 512 channels with a residual 230 and 252.)
+        const int stage = room >= 2 * NA_STAGE_BYTES ? NA_STAGE_BYTES : room / 3;
+        p.tile_rows = lanes * std::max(1, stage / (lanes * row_bytes * tensors));
         p.sums_tile_rows = BACKWARD ? p.tile_rows : p.tile_rows * tensors;
         p.stage_bytes = (p.tile_rows * row_bytes * tensors + 127) / 128 * 128;
-        p.stages = std::min(RING_STAGES, (NA_RING_BYTES - (int)ring_bytes(p.V, p.G, BACKWARD)) / p.stage_bytes);
+        p.stages = std::min(RING_STAGES, room / p.stage_bytes);
         if (p.stages < 2) p.stages = 0;
     }
     if (!p.stages) p.phase_bits = 0;

@@ -26,9 +26,9 @@
 // Tickets are ordered so that a sample is applied some chunks after its sums, in the hope that the wait for them is over by then.
 //
 // What is summed:
-//   forward   mean and sum of squares about it.  A block sums x - k and its square, k the channel's value in the piece's first row
-//             (or next to it, see shift_of): as k is one of the n summed values, (k - mean)^2 is at most their sum of squares M2, and what cancels in
-//             sum (x - k)^2 - n (mean - k)^2 is at most (n + 1) M2: n + 1 roundings at worst, one where rows are alike.
+//   forward   mean and sum of squares about it.  A block sums x - k and its square, k next to the channel's mean over some of the
+//             piece's n rows (see shift_of): as k is the mean of m of the summed values, m (k - mean)^2 is at most their sum of squares M2, and what
+//             cancels in sum (x - k)^2 - n (mean - k)^2 is at most (n / m + 1) M2: so many roundings at worst, some two where rows are alike.
 //   backward  gz and gz * xh.
 #pragma once
 #include <algorithm>
@@ -487,11 +487,30 @@ struct Rows {
     }
 };
 
-// What is taken off the values that are squared and summed: the first of them.  Values of 16 bits are multiples of a power of two, the
-// square of an odd multiple is 1 modulo 8, and so what does not fit a sum's 24 bits is rounded down nearly always: 4e-8 of the sum of squares,
-// however many rows.  A value a little beside theirs has no such pattern.  (Beside by 2^-11 of it: 16-bit values differ by more.)
+// What is taken off the values that are squared and summed: the mean of SHIFT_ROWS of them (of what there is, where that is less).  (Of the
+// first alone, statistics of a thousand rows were 9e-8 of a deviation off, 8e-7 at most: what it is beside the mean is in every term.)
+// Values of 16 bits are multiples of a power of two, the square of an odd multiple is 1 modulo 8, and so what does not fit a sum's 24 bits
+// is rounded down nearly always: 4e-8 of the sum of squares, however many rows.  A value a little beside theirs has no such
+// pattern.  (Beside by 2^-11 of it: 16-bit values differ by more.)
+constexpr int SHIFT_ROWS = 8;
 template <typename T>
-__device__ __forceinline__ float shift_of(float first) { return sizeof(T) == 4 ? first : first * 1.000457f; }
+__device__ __forceinline__ float shift_of(float middle) { return sizeof(T) == 4 ? middle : middle * 1.000457f; }
+// -shift of a lump's channels, `row(j)` the j-th of m rows.
+template <typename T, int VN, typename Row>
+__device__ __forceinline__ void minus_shift(int m, float2 *k, Row row) {
+    constexpr int P = (VN + 1) / 2;
+    const float share = 1.f / (float)m;
+#pragma unroll
+    for (int j = 0; j < P; ++j) k[j] = both(0.f);
+#pragma unroll 4
+    for (int i = 0; i < m; ++i) {
+        const Lump<T, VN> v = row(i);
+#pragma unroll
+        for (int j = 0; j < P; ++j) k[j] = fma2(pair_of(v, j), both(share), k[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < P; ++j) k[j] = make_float2(-shift_of<T>(k[j].x), -shift_of<T>(k[j].y));
+}
 
 template <typename T, int VN>
 __device__ __forceinline__ void stats_piece(const NormAct &p, const Columns &l, int64_t piece, int64_t lo, int n, float2 *fold) {
@@ -504,14 +523,16 @@ __device__ __forceinline__ void stats_piece(const NormAct &p, const Columns &l, 
         for (int j = 0; j < P; ++j) a[j] = b[j] = both(0.f);
         if (lump < l.lumps && l.lane < l.lanes) {
             const T *col = x + (int64_t)lump * VN;
-            Lump<T, VN> first;
-            first.load(col);
             int r = l.lane;
             Rows<T, VN, U> in;
             in.load(col, r, n, l.lanes, p.C);
             float2 k[P];
-#pragma unroll
-            for (int j = 0; j < P; ++j) k[j] = make_float2(-shift_of<T>(pair_of(first, j).x), -shift_of<T>(pair_of(first, j).y));
+            const int m = min(n, SHIFT_ROWS);
+            minus_shift<T, VN>(m, k, [&](int i) {
+                Lump<T, VN> v;
+                v.load(col + (int64_t)(i * n / m) * p.C);
+                return v;
+            });
             for (; r < n; r += U * l.lanes) {
 #pragma unroll
                 for (int u = 0; u < U; ++u)
@@ -526,7 +547,14 @@ __device__ __forceinline__ void stats_piece(const NormAct &p, const Columns &l, 
         }
         fold_lanes<VN>(l, pass, a, b, fold, [&](int c, float sa, float sb) {
             const float off = sa / (float)n;
-            p.rec[piece * p.C + c] = make_float2(shift_of<T>(to_f32<T>(x[c])) + off, fmaxf(sb - sa * off, 0.f));
+            const int m = min(n, SHIFT_ROWS);
+            float2 k;   // (the same again)
+            minus_shift<T, 1>(m, &k, [&](int i) {
+                Lump<T, 1> v;
+                v.load(x + (int64_t)(i * n / m) * p.C + c);
+                return v;
+            });
+            p.rec[piece * p.C + c] = make_float2(off - k.x, fmaxf(sb - sa * off, 0.f));
         });
     }
 }
@@ -955,7 +983,7 @@ struct Ring {
     Piece pieces[FOLD_SLOTS];
     int told, abort;
 };
-// (behind the ring's tiles) two slots of sums, the channels' values in the piece's first row for each, constants
+// (behind the ring's tiles) two slots of sums, what is taken off the channels' values for each, constants
 struct RingMemory {
     char *stages;
     float2 *fold;
@@ -1245,20 +1273,29 @@ __device__ __forceinline__ void ring_worker(const NormAct &p, Ring &ring, const 
             if constexpr (BACKWARD) {
                 k_sums.read_all(l, K_MU, k), k_sums.read_all(l, K_A, fa), k_sums.read_all(l, K_B, fb);
             } else {
-                Lump<T, VN> v;   // of the piece's first row
                 if constexpr (PHASES) {
-                    const T *row = rows_at() - c0 + ends().x;
-                    int c = channel_of(p, c0);
+                    const int2 e = ends();
+                    const T *tile = rows_at() - c0 + e.x;
+                    const int n = (e.y - e.x) / p.C, m = min(n, SHIFT_ROWS), first = channel_of(p, c0);
+                    minus_shift<T, VN>(m, k, [&](int row) {
+                        Lump<T, VN> v;
+                        const T *from = tile + row * n / m * p.C;
+                        int c = first;
 #pragma unroll
-                    for (int i = 0; i < VN; ++i) {
-                        v.set(i, to_f32<T>(row[c]));
-                        if (++c == p.C) c = 0;
-                    }
+                        for (int i = 0; i < VN; ++i) {
+                            v.set(i, to_f32<T>(from[c]));
+                            if (++c == p.C) c = 0;
+                        }
+                        return v;
+                    });
                 } else {
-                    v.load(rows_at());
+                    const int m = min(t.n, SHIFT_ROWS);
+                    minus_shift<T, VN>(m, k, [&](int row) {
+                        Lump<T, VN> v;
+                        v.load(rows_at() + row * t.n / m * p.V);
+                        return v;
+                    });
                 }
-#pragma unroll
-                for (int j = 0; j < P; ++j) k[j] = make_float2(-shift_of<T>(pair_of(v, j).x), -shift_of<T>(pair_of(v, j).y));
                 if (l.lane == 0 && free) {   // (C of V are read)
 #pragma unroll
                     for (int j = 0; j < P; ++j) *reinterpret_cast<float2 *>(m.firsts + slot.at * p.V + c0 + 2 * j) = neg2(k[j]);
