@@ -793,9 +793,10 @@ __device__ __forceinline__ int lanes_of_group(const NormAct &p) {
     return share;
 }
 
-// The records of a piece's groups, of `n` rows, from its channels' (`channel(c)`, visible to the team).
-template <bool BACKWARD, typename Team, typename Channel>
-__device__ __forceinline__ void group_records(const NormAct &p, int share, int64_t piece, int n, Channel channel) {
+// The records of a piece's groups, of `n` rows, from its channels' (`channel(c)`, visible to the team; forward the mean beside `base(c)`:
+// the sum of the two in one float would be rounded by more than all that was summed).
+template <bool BACKWARD, typename Team, typename Channel, typename Base>
+__device__ __forceinline__ void group_records(const NormAct &p, int share, int64_t piece, int n, Channel channel, Base base) {
     const int l = Team::rank() % share;
     const auto sum = [&](float v) {
         for (int o = share / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -815,18 +816,18 @@ __device__ __forceinline__ void group_records(const NormAct &p, int share, int64
             a = sum(a), b = sum(b);
             if (g < p.G && l == 0) to[g] = {a, b};
         } else {   // the mean about the first channel's, then squares about it
-            const float k = channel(c0).x;
+            const float k = channel(c0).x, from = base(c0);
 #pragma unroll 4
-            for (int i = l; i < end; i += share) a += channel(c0 + i).x - k;
+            for (int i = l; i < end; i += share) a += (base(c0 + i) - from) + (channel(c0 + i).x - k);
             const float off = sum(a) / (float)p.W;
 #pragma unroll 4
             for (int i = l; i < end; i += share) {
                 const float2 v = channel(c0 + i);
-                const float d = (v.x - k) - off;
+                const float d = ((base(c0 + i) - from) + (v.x - k)) - off;
                 b += v.y + (float)n * d * d;
             }
             b = sum(b);
-            const double mean = (double)k + off;
+            const double mean = ((double)from + k) + off;
             if (g < p.G && l == 0) to[g] = {(float)mean, (float)(mean - (double)(float)mean), b, 0.f};
         }
     }
@@ -933,7 +934,7 @@ __global__ void __launch_bounds__(NA_THREADS, BACKWARD ? 3 : 4) na_kernel(const 
                 else stats_piece<T, VN>(p, l, chunk + s, lo, (int)(hi - lo), fold);
                 sync_workers();
                 const float2 *channels = p.rec + (chunk + s) * p.C;   // (what this block has written)
-                group_records<BACKWARD, BlockTeam>(p, lanes_of_group<BlockTeam>(p), chunk + s, (int)(hi - lo), [&](int c) { return __ldcg(channels + c); });
+                group_records<BACKWARD, BlockTeam>(p, lanes_of_group<BlockTeam>(p), chunk + s, (int)(hi - lo), [&](int c) { return __ldcg(channels + c); }, [](int) { return 0.f; });
                 count_piece<BACKWARD, BlockTeam>(p, p.spans[s], chunk, s, &told);
             } else {
                 bool there;
@@ -1156,12 +1157,12 @@ __device__ __forceinline__ void ring_clerk(const NormAct &p, Ring &ring, const R
                 if (p.dweight) p.rec[number * p.C + c] = make_float2(a, b);
             } else {
                 const float off = a / (float)piece.rows;   // (not by a rounded inverse: its error is the same in every piece)
-                b = fmaxf(b - a * off, 0.f), a = firsts[c] + off;
+                b = fmaxf(b - a * off, 0.f), a = off;
             }
             fold[c % 8 * FOLD_STRIDE + c / 8] = make_float2(a, b);
         }
         __syncwarp();
-        group_records<BACKWARD, WarpTeam>(p, share, number, piece.rows, [&](int c) { return fold[c % 8 * FOLD_STRIDE + c / 8]; });
+        group_records<BACKWARD, WarpTeam>(p, share, number, piece.rows, [&](int c) { return fold[c % 8 * FOLD_STRIDE + c / 8]; }, [&](int c) { return firsts[c]; });
         __syncwarp();
         if (lane == 0) tc::mbar_arrive(tc::smem_u32(&ring.taken[slot.at]));
         count_piece<BACKWARD, WarpTeam>(p, p.spans[piece.s], piece.chunk, piece.s, &ring.told);
