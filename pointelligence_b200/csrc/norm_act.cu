@@ -124,11 +124,12 @@ size_t carve(void *ws, int64_t N, int64_t S, int C, int G, int dtype, NormAct *o
     p.chunks = (int)((N + p.rows - 1) / p.rows);
     p.offsets = c.take<int64_t>((size_t)S + 1);
     p.spans = c.take<Span>((size_t)S);
-    p.rec = c.take<float2>((size_t)(p.chunks + S) * C);
+    p.rec = c.take<float2>(std::max((size_t)(p.chunks + S) * C, (size_t)std::min<int64_t>(2 * (int64_t)p.chunks, NA_BLOCKS * num_sms()) * C * 2));
+    p.scratch = reinterpret_cast<double2 *>(p.rec);   // (forward; the other is backward)
     p.window = window_of(p.chunks, G);
     const size_t windows = p.window > 1 ? (size_t)windows_in_all(p.chunks, S, p.window) : 0;
-    p.of_piece = c.take<float4>((size_t)(p.chunks + S) * G);   // (backward: of float2)
-    p.of_window = windows ? c.take<float4>(windows * G) : p.of_piece;
+    p.of_piece = c.take<double2>((size_t)(p.chunks + S) * G);   // (backward: of float2)
+    p.of_window = windows ? c.take<double2>(windows * G) : p.of_piece;
     p.control = c.take<int>(CONTROL_WORDS + (size_t)S + windows);
     if (out) *out = p;
     return c.off;

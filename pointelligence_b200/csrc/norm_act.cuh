@@ -10,12 +10,14 @@
 //   gz = drop'(g) * act'(z),   dresidual = gz,   dbias[c] = sum over rows of gz,   dweight[c] = sum over rows of gz * xh,
 //   gh = gz * weight,   dx = rstd * (gh - sum_{s,g}(gh) / n - xh * sum_{s,g}(gh * xh) / n).
 //
-// Everything is held in fp32 between one read of an element and its one rounding.
+// Everything is held in fp32 between one read of an element and its one rounding, but for the statistics, which are fp64 from the element
+// on: the sign of a ReLU's argument hangs on them, and where 32 bits summed them (1e-8 of a deviation off), about one of 70 million
+// elements came out on the other side, each of which moves dbias by a whole gradient.
 //
 // Both directions take two passes over the rows, with sums between them, in one launch (behind a small one that lays the samples
 // out).  A chunk is `rows` consecutive rows; a piece is what a chunk has of one sample, piece chunk + s (pieces are ordered, and
 // the next one has a higher chunk or a higher sample by one).  Blocks take tickets, in ascending order, one at a time:
-//   sums of a chunk  two floats per channel and piece, whatever the group's width, and from them two per group
+//   sums of a chunk  two sums per channel and piece, whatever the group's width, and from them two per group
 //   apply of a chunk the second pass, once the sums of its samples are there
 //   affine           dweight and dbias of some channels, once those of all samples are
 // A sample's records of groups are merged by every block that applies rows of it, for itself: one turn through the L2 from the last
@@ -26,9 +28,9 @@
 // Tickets are ordered so that a sample is applied some chunks after its sums, in the hope that the wait for them is over by then.
 //
 // What is summed:
-//   forward   mean and sum of squares about it.  A block sums x - k and its square, k next to the channel's mean over some of the
-//             piece's n rows (see shift_of): as k is the mean of m of the summed values, m (k - mean)^2 is at most their sum of squares M2, and what
-//             cancels in sum (x - k)^2 - n (mean - k)^2 is at most (n / m + 1) M2: so many roundings at worst, some two where rows are alike.
+//   forward   mean and sum of squares about it.  A block sums x - k and its square, k the channel's value in the piece's first row:
+//             as k is one of the n summed values, (k - mean)^2 is at most their sum of squares M2, and what cancels in
+//             sum (x - k)^2 - n (mean - k)^2 is at most (n + 1) M2: n + 1 roundings of 2^-53 at worst.
 //   backward  gz and gz * xh.
 #pragma once
 #include <algorithm>
@@ -41,6 +43,7 @@
 namespace pcx {
 
 constexpr int NA_THREADS = 256;
+constexpr int NA_BLOCKS = 3;          // of the kernel without the ring, on a multiprocessor
 constexpr unsigned NA_STATUS = 32u;   // of a wait that ran out
 constexpr int AFFINE_CHANNELS = 8;    // of a ticket
 enum { TICKET = 0, WINDOWS_DONE = 1, WINDOWS = 2, CONTROL_WORDS = 4 };
@@ -58,7 +61,8 @@ struct NormAct {
     float *dweight, *dbias;
     int64_t *offsets;              // (S + 1)
     Span *spans;                   // (S)
-    float2 *rec;                   // (pieces, C): mean and M2; or sums of gz and gz * xh
+    float2 *rec;                   // backward (pieces, C): sums of gz and gz * xh
+    double2 *scratch;              // forward, without the ring (blocks, C): mean and M2 of the piece that a block is at
     void *of_piece, *of_window;    // (pieces, G), (windows, G) of Record: the same of groups, the sums with the channels' weights
     int *control;                  // the words above, then windows that each sample has, pieces that each window has
     unsigned int *status;
@@ -204,13 +208,14 @@ __device__ __forceinline__ bool sync_workers_and(bool v) {
     return all != 0;
 }
 
-// What a piece leaves of a group.  Forward: mean and M2, the mean in two floats: rounded to one, it would make the activation's argument
-// uncertain by 2^-25 of it, and with it the sign that decides the ReLU's gradient: of 70 million elements about one came out on the
-// other side, each of which moves dbias by a whole gradient.  (Roundings further down are many, and average out.)
+// Below zero, by roundings, is zero; a NaN stays one.
+__device__ __forceinline__ double not_below_zero(double v) { return v < 0.0 ? 0.0 : v; }
+
+// What a piece leaves of a group.  Forward: mean and M2.
 template <bool BACKWARD>
 struct Record;
 template <>
-struct __align__(16) Record<false> { float mean, low, m2, none; };
+struct __align__(16) Record<false> { double mean, m2; };
 template <>
 struct __align__(8) Record<true> { float x, y; };
 __device__ __forceinline__ Record<true> load_record(const Record<true> *p) {
@@ -218,33 +223,33 @@ __device__ __forceinline__ Record<true> load_record(const Record<true> *p) {
     return {v.x, v.y};
 }
 __device__ __forceinline__ Record<false> load_record(const Record<false> *p) {
-    const float4 v = __ldcg(reinterpret_cast<const float4 *>(p));
-    return {v.x, v.y, v.z, 0.f};
+    const double2 v = __ldcg(reinterpret_cast<const double2 *>(p));
+    return {v.x, v.y};
 }
 
-// Records that follow one another: `count` of `unit` rows each, but for the first and the last.
+// Records that follow one another: `count` of `unit` elements each, but for the first and the last.
 template <bool BACKWARD>
 struct Records {
     const Record<BACKWARD> *at;
     int count;
-    float first, unit, last;   // rows
+    double first, unit, last;
     double inverse;            // 1 / elements of all of them
 };
 // Rows lo .. hi by spans of `unit` rows, the first of which begins at `from`; `each` elements a row.
 template <bool BACKWARD>
 __device__ __forceinline__ Records<BACKWARD> records_of(const void *at, int64_t first, int count, int64_t lo, int64_t hi, int64_t from, int64_t unit, int each) {
-    return {static_cast<const Record<BACKWARD> *>(at) + first, count, (float)(min(hi, from + unit) - lo), (float)unit, (float)(hi - (from + (count - 1) * unit)),
-            1.0 / ((double)(hi - lo) * each)};
+    return {static_cast<const Record<BACKWARD> *>(at) + first, count, (double)((min(hi, from + unit) - lo) * each), (double)(unit * each),
+            (double)((hi - (from + (count - 1) * unit)) * each), 1.0 / ((double)(hi - lo) * each)};
 }
 
-// Sums over records, of which a thread has some.  Forward all are differences from the first record, or squares of them, so that what
-// is rounded is small: a, b of means and their squares, m2 of M2.  Backward: of both sums.
+// Sums over records, of which a thread has some.  Forward about the first record's mean: a of differences from it, b of squares, each
+// record's own among them.  Backward: of both sums.
 template <bool BACKWARD>
 struct RecordSums;
 template <>
 struct RecordSums<true> {
     static constexpr int AHEAD = 8;   // loads at once
-    float a = 0.f, b = 0.f, m2 = 0.f;
+    float a = 0.f, b = 0.f;
     __device__ __forceinline__ void add(const Records<true> &r, int stride, int g, int q, int deep) {
         const Record<true> *at = r.at + g;
         for (int i = q; i < r.count; i += AHEAD * deep) {
@@ -255,46 +260,32 @@ struct RecordSums<true> {
             for (int u = 0; u < AHEAD; ++u) a += v[u].x, b += v[u].y;
         }
     }
-    __device__ __forceinline__ Record<true> done(const Records<true> &, int) const { return {a, b}; }
+    __device__ __forceinline__ Record<true> done(const Records<true> &) const { return {a, b}; }
 };
 template <>
 struct RecordSums<false> {
     static constexpr int AHEAD = 8;
-    float a = 0.f, b = 0.f, m2 = 0.f;
-    Record<false> k, last;
-    __device__ __forceinline__ float away(const Record<false> &v) const { return (v.mean - k.mean) + (v.low - k.low); }
+    double a = 0.0, b = 0.0, k = 0.0;
     __device__ __forceinline__ void add(const Records<false> &r, int stride, int g, int q, int deep) {
         const Record<false> *at = r.at + g;
-        k = load_record(at), last = load_record(at + (int64_t)(r.count - 1) * stride);
+        k = load_record(at).mean;
         for (int i = q; i < r.count; i += AHEAD * deep) {
             Record<false> v[AHEAD];
 #pragma unroll
-            for (int u = 0; u < AHEAD; ++u) v[u] = i + u * deep < r.count ? load_record(at + (int64_t)(i + u * deep) * stride) : k;
+            for (int u = 0; u < AHEAD; ++u) v[u] = i + u * deep < r.count ? load_record(at + (int64_t)(i + u * deep) * stride) : Record<false>{k, 0.0};
 #pragma unroll
             for (int u = 0; u < AHEAD; ++u) {
-                const float d = away(v[u]);
-                a += d, b += d * d, m2 += v[u].m2 - k.m2;
+                const int j = i + u * deep;
+                const double n = j == 0 ? r.first : j == r.count - 1 ? r.last : r.unit, d = v[u].mean - k, nd = n * d;
+                a += nd, b += fma(nd, d, v[u].m2);
             }
         }
     }
-    struct Moments { double mean, m2; };
-    __device__ __forceinline__ Moments moments(const Records<false> &r, int each) const {   // (the first record's rows do not matter to a and b, the last's do)
-        const double d = away(last), less = (double)r.unit - r.last;
-        const double sum = ((double)r.unit * a - less * d) * each, off = sum * r.inverse;
-        const double squares = ((double)r.unit * b - less * d * d) * each - sum * off;
-        return {((double)k.mean + k.low) + off, fmax(((double)r.count * k.m2 + m2) + squares, 0.0)};
-    }
-    __device__ __forceinline__ Record<false> done(const Records<false> &r, int each) const {
-        const Moments v = moments(r, each);
-        return {(float)v.mean, (float)(v.mean - (double)(float)v.mean), (float)v.m2, 0.f};
+    __device__ __forceinline__ Record<false> done(const Records<false> &r) const {
+        const double off = a * r.inverse;
+        return {k + off, not_below_zero(fma(-a, off, b))};
     }
 };
-
-// 1 / sqrt(v), from fp32's by a step of Newton's
-__device__ __forceinline__ double rsqrt_of(double v) {
-    const double y = rsqrtf((float)v);
-    return y * (1.5 - 0.5 * v * y * y);
-}
 
 // What a second pass needs of the groups that channels c0 .. c1 - 1 are in, from the sample's records, into `stats` (shared memory) by all
 // workers: mean and rstd, or the backward's two means.  Every block does this for itself, with the sample's windows counted: a block
@@ -302,7 +293,7 @@ __device__ __forceinline__ double rsqrt_of(double v) {
 // there are fewer of them, in rows on the records.
 struct Stats { double x, y; };
 template <bool BACKWARD>
-__device__ __forceinline__ void merge_groups(const NormAct &p, const Records<BACKWARD> &r, int groups, Stats *stats, float4 *scratch) {
+__device__ __forceinline__ void merge_groups(const NormAct &p, const Records<BACKWARD> &r, int groups, Stats *stats, double2 *scratch) {
     const int wide = min(groups, NA_THREADS), at = threadIdx.x % wide, q = threadIdx.x / wide;
     const bool shuffles = wide < 32 && 32 % wide == 0;
     const int deep = NA_THREADS / wide;
@@ -313,26 +304,25 @@ __device__ __forceinline__ void merge_groups(const NormAct &p, const Records<BAC
         if (shuffles) {   // a warp's rows first; then its first row has them
             for (int o = 16; o >= wide; o >>= 1) {
                 sums.a += __shfl_xor_sync(0xffffffffu, sums.a, o), sums.b += __shfl_xor_sync(0xffffffffu, sums.b, o);
-                if (!BACKWARD) sums.m2 += __shfl_xor_sync(0xffffffffu, sums.m2, o);
             }
         }
         const int rows = shuffles ? NA_THREADS / 32 : deep, step = shuffles ? 32 : wide;
         if (rows > 1) {
-            scratch[threadIdx.x] = make_float4(sums.a, sums.b, sums.m2, 0.f);
+            scratch[threadIdx.x] = make_double2(sums.a, sums.b);
             sync_workers();
             if (q == 0)
 #pragma unroll 4
                 for (int i = 1; i < rows; ++i) {
-                    const float4 v = scratch[i * step + at];
-                    sums.a += v.x, sums.b += v.y, sums.m2 += v.z;
+                    const double2 v = scratch[i * step + at];
+                    sums.a += v.x, sums.b += v.y;
                 }
         }
         if (g < groups && q == 0) {
             if constexpr (BACKWARD) {
                 stats[g] = {sums.a * r.inverse, sums.b * r.inverse};
             } else {
-                const auto v = sums.moments(r, p.W);
-                stats[g] = {v.mean, rsqrt_of(v.m2 * r.inverse + p.eps)};
+                const Record<false> v = sums.done(r);
+                stats[g] = {v.mean, rsqrt(v.m2 * r.inverse + p.eps)};
             }
         }
         sync_workers();
@@ -370,7 +360,7 @@ struct Constants {
     static constexpr int QUAD = VN < 4 ? VN : 4, PAIRS = QUAD < 2 ? 1 : QUAD / 2, QUADS = VN / QUAD;
     float *at;
     Stats *stats;              // of the second pass: the groups'
-    float4 *scratch;           // of merge_groups
+    double2 *scratch;          // of merge_groups
     int64_t s = -1;            // whose they are
     int pass = -1;
     __device__ __forceinline__ void read(const Columns &l, int k, int h, float2 *out) const {
@@ -432,45 +422,47 @@ struct Constants {
 };
 
 // ------------------------------------------------------------ sums of a piece ----
-// Sums of entries q, q + step, .. of `lanes` that are `stride` apart, in eight chains: one of all of them (85 lanes of four rows side by
-// side, for 6 channels) rounds by 1e-6 of a deviation, ten times what the rest of the statistics do.
+// Sums of entries q, q + step, .. of `lanes` that are `stride` apart, in eight chains: they do not wait for one another's additions, and
+// one chain of 32 bits of all of them (85 lanes of four rows side by side, for 6 channels) rounds by 1e-6 of a gradient's size.
+template <typename Two>
 struct Chains {
-    float2 part[8];
+    Two part[8];
     __device__ __forceinline__ Chains() {
 #pragma unroll
-        for (int u = 0; u < 8; ++u) part[u] = make_float2(0.f, 0.f);
+        for (int u = 0; u < 8; ++u) part[u] = Two{};
     }
-    __device__ __forceinline__ void add(const float2 *from, int q, int step, int lanes, int stride) {
+    __device__ __forceinline__ void add(const Two *from, int q, int step, int lanes, int stride) {
         for (; q < lanes; q += 8 * step) {
 #pragma unroll
             for (int u = 0; u < 8; ++u)
                 if (q + u * step < lanes) {
-                    const float2 v = from[(q + u * step) * stride];
+                    const Two v = from[(q + u * step) * stride];
                     part[u].x += v.x, part[u].y += v.y;
                 }
         }
     }
-    __device__ __forceinline__ float2 sum() const {
-        float2 v[4];
+    __device__ __forceinline__ Two sum() const {
+        Two v[4];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) v[u] = make_float2(part[u].x + part[u + 4].x, part[u].y + part[u + 4].y);
-        return make_float2((v[0].x + v[1].x) + (v[2].x + v[3].x), (v[0].y + v[1].y) + (v[2].y + v[3].y));
+        for (int u = 0; u < 4; ++u) v[u].x = part[u].x + part[u + 4].x, v[u].y = part[u].y + part[u + 4].y;
+        Two all;
+        all.x = (v[0].x + v[1].x) + (v[2].x + v[3].x), all.y = (v[0].y + v[1].y) + (v[2].y + v[3].y);
+        return all;
     }
 };
 
-// Two sums per channel of a thread's rows, folded over the block's row lanes; `out(c, a, b)` for every channel.
-template <int VN, typename Out>
-__device__ __forceinline__ void fold_lanes(const Columns &l, int pass, const float2 *a, const float2 *b, float2 *fold, Out out) {
+// Two sums per channel of a thread's rows (`part(i)`), folded over the block's row lanes; `out(c, a, b)` for every channel.
+template <int VN, typename Two, typename Part, typename Out>
+__device__ __forceinline__ void fold_lanes(const Columns &l, int pass, Two *fold, Part part, Out out) {
     sync_workers();   // (the piece before has been read)
 #pragma unroll
-    for (int i = 0; i < VN; ++i)
-        fold[i * NA_THREADS + threadIdx.x] = i % 2 ? make_float2(a[i / 2].y, b[i / 2].y) : make_float2(a[i / 2].x, b[i / 2].x);
+    for (int i = 0; i < VN; ++i) fold[i * NA_THREADS + threadIdx.x] = part(i);
     sync_workers();
     for (int t = threadIdx.x; t < l.cols * VN; t += NA_THREADS) {
         const int i = t / l.cols, col = t % l.cols, lump = pass * l.cols + col;
-        Chains chains;
+        Chains<Two> chains;
         chains.add(fold + i * NA_THREADS + col, 0, 1, l.lanes, l.cols);
-        const float2 v = chains.sum();
+        const Two v = chains.sum();
         if (lump < l.lumps) out(lump * VN + i, v.x, v.y);
     }
 }
@@ -487,74 +479,54 @@ struct Rows {
     }
 };
 
-// What is taken off the values that are squared and summed: the mean of SHIFT_ROWS of them (of what there is, where that is less).  (Of the
-// first alone, statistics of a thousand rows were 9e-8 of a deviation off, 8e-7 at most: what it is beside the mean is in every term.)
-// Values of 16 bits are multiples of a power of two, the square of an odd multiple is 1 modulo 8, and so what does not fit a sum's 24 bits
-// is rounded down nearly always: 4e-8 of the sum of squares, however many rows.  A value a little beside theirs has no such
-// pattern.  (Beside by 2^-11 of it: 16-bit values differ by more.)
-constexpr int SHIFT_ROWS = 8;
-template <typename T>
-__device__ __forceinline__ float shift_of(float middle) { return sizeof(T) == 4 ? middle : middle * 1.000457f; }
-// -shift of a lump's channels, `row(j)` the j-th of m rows.
-template <typename T, int VN, typename Row>
-__device__ __forceinline__ void minus_shift(int m, float2 *k, Row row) {
-    constexpr int P = (VN + 1) / 2;
-    const float share = 1.f / (float)m;
+// Sums of a channel's x - k and of their squares, k its value in the piece's first row: 64 bits a rounding, from the element on.
+template <int VN>
+struct Moments {
+    double a[VN], b[VN], k[VN];
+    template <typename T>
+    __device__ __forceinline__ explicit Moments(const Lump<T, VN> &first) {
 #pragma unroll
-    for (int j = 0; j < P; ++j) k[j] = both(0.f);
-#pragma unroll 4
-    for (int i = 0; i < m; ++i) {
-        const Lump<T, VN> v = row(i);
-#pragma unroll
-        for (int j = 0; j < P; ++j) k[j] = fma2(pair_of(v, j), both(share), k[j]);
+        for (int i = 0; i < VN; ++i) a[i] = b[i] = 0.0, k[i] = first.get(i);
     }
+    // Of a lump, the elements first <= i < end.
+    template <typename T>
+    __device__ __forceinline__ void add(const Lump<T, VN> &v, int first = 0, int end = VN) {
 #pragma unroll
-    for (int j = 0; j < P; ++j) k[j] = make_float2(-shift_of<T>(k[j].x), -shift_of<T>(k[j].y));
+        for (int i = 0; i < VN; ++i) {
+            const double d = i >= first && i < end ? (double)v.get(i) - k[i] : 0.0;
+            a[i] += d, b[i] = fma(d, d, b[i]);
+        }
+    }
+};
+// The mean and M2 of n values, of which a and b are the sums about k.
+__device__ __forceinline__ double2 moments_of(double k, double a, double b, double inverse) {
+    const double off = a * inverse;
+    return make_double2(k + off, not_below_zero(fma(-a, off, b)));
 }
 
 template <typename T, int VN>
-__device__ __forceinline__ void stats_piece(const NormAct &p, const Columns &l, int64_t piece, int64_t lo, int n, float2 *fold) {
-    constexpr int U = sizeof(T) == 4 && VN == 8 ? 2 : 4, P = (VN + 1) / 2;
+__device__ __forceinline__ void stats_piece(const NormAct &p, const Columns &l, int64_t lo, int n, double2 *fold) {
+    constexpr int U = VN == 8 ? 2 : 4;
     const T *x = static_cast<const T *>(p.x) + lo * p.C;
+    const double inverse = 1.0 / (double)n;
     for (int pass = 0; pass < l.passes; ++pass) {
         const int lump = pass * l.cols + l.col;
-        float2 a[P], b[P];
+        const bool mine = lump < l.lumps && l.lane < l.lanes;
+        const T *col = x + (int64_t)(mine ? lump : 0) * VN;
+        int r = mine ? l.lane : n;
+        Rows<T, VN, U> in;
+        in.load(col, r, n, l.lanes, p.C);
+        Lump<T, VN> k;
+        k.load(col);
+        Moments<VN> sums(k);
+        for (; r < n; r += U * l.lanes) {
 #pragma unroll
-        for (int j = 0; j < P; ++j) a[j] = b[j] = both(0.f);
-        if (lump < l.lumps && l.lane < l.lanes) {
-            const T *col = x + (int64_t)lump * VN;
-            int r = l.lane;
-            Rows<T, VN, U> in;
-            in.load(col, r, n, l.lanes, p.C);
-            float2 k[P];
-            const int m = min(n, SHIFT_ROWS);
-            minus_shift<T, VN>(m, k, [&](int i) {
-                Lump<T, VN> v;
-                v.load(col + (int64_t)(i * n / m) * p.C);
-                return v;
-            });
-            for (; r < n; r += U * l.lanes) {
-#pragma unroll
-                for (int u = 0; u < U; ++u)
-                    if (r + u * l.lanes < n)
-#pragma unroll
-                        for (int j = 0; j < P; ++j) {
-                            const float2 d = add2(pair_of(in.v[u], j), k[j]);
-                            a[j] = add2(a[j], d), b[j] = fma2(d, d, b[j]);
-                        }
-                in.load(col, r + U * l.lanes, n, l.lanes, p.C);
-            }
+            for (int u = 0; u < U; ++u)
+                if (r + u * l.lanes < n) sums.add(in.v[u]);
+            in.load(col, r + U * l.lanes, n, l.lanes, p.C);
         }
-        fold_lanes<VN>(l, pass, a, b, fold, [&](int c, float sa, float sb) {
-            const float off = sa / (float)n;
-            const int m = min(n, SHIFT_ROWS);
-            float2 k;   // (the same again)
-            minus_shift<T, 1>(m, &k, [&](int i) {
-                Lump<T, 1> v;
-                v.load(x + (int64_t)(i * n / m) * p.C + c);
-                return v;
-            });
-            p.rec[piece * p.C + c] = make_float2(off - k.x, fmaxf(sb - sa * off, 0.f));
+        fold_lanes<VN>(l, pass, fold, [&](int i) { return make_double2(sums.a[i], sums.b[i]); }, [&](int c, double a, double b) {
+            p.scratch[(int64_t)blockIdx.x * p.C + c] = moments_of(to_f32<T>(x[c]), a, b, inverse);
         });
     }
 }
@@ -711,7 +683,7 @@ __device__ __forceinline__ void bwd_sums_piece(const NormAct &p, const Columns &
             }
             in.load(p, l, from, r + U * l.lanes, n);
         }
-        fold_lanes<VN>(l, pass, a, b, fold, [&](int c, float sa, float sb) {
+        fold_lanes<VN>(l, pass, fold, [&](int i) { return i % 2 ? make_float2(a[i / 2].y, b[i / 2].y) : make_float2(a[i / 2].x, b[i / 2].x); }, [&](int c, float sa, float sb) {
             p.rec[piece * p.C + c] = make_float2(sa, sb * (float)__ldg(p.rstd + s * p.G + group_of(p, c)));
         });
     }
@@ -781,7 +753,7 @@ __device__ __forceinline__ void merge_window(const NormAct &p, const Records<BAC
     for (int g = Team::rank(); g < p.G; g += Team::SIZE) {
         RecordSums<BACKWARD> sums;
         sums.add(r, p.G, g, 0, 1);
-        to[g] = sums.done(r, p.W);
+        to[g] = sums.done(r);
     }
 }
 
@@ -793,20 +765,20 @@ __device__ __forceinline__ int lanes_of_group(const NormAct &p) {
     return share;
 }
 
-// The records of a piece's groups, of `n` rows, from its channels' (`channel(c)`, visible to the team; forward the mean beside `base(c)`:
-// the sum of the two in one float would be rounded by more than all that was summed).
-template <bool BACKWARD, typename Team, typename Channel, typename Base>
-__device__ __forceinline__ void group_records(const NormAct &p, int share, int64_t piece, int n, Channel channel, Base base) {
+// The records of a piece's groups, of `n` rows, from its channels' (`channel(c)`, visible to the team).
+template <bool BACKWARD, typename Team, typename Channel>
+__device__ __forceinline__ void group_records(const NormAct &p, int share, int64_t piece, int n, Channel channel) {
     const int l = Team::rank() % share;
-    const auto sum = [&](float v) {
+    const auto sum = [&](auto v) {
         for (int o = share / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
         return v;
     };
     Record<BACKWARD> *to = static_cast<Record<BACKWARD> *>(p.of_piece) + piece * p.G;
+    const double inverse = 1.0 / p.W;
     for (int g0 = 0; g0 < p.G; g0 += Team::SIZE / share) {   // (the same rounds for all lanes of a warp)
         const int g = g0 + Team::rank() / share, c0 = min(g, p.G - 1) * p.W, end = g < p.G ? p.W : 0;
-        float a = 0.f, b = 0.f;
         if constexpr (BACKWARD) {
+            float a = 0.f, b = 0.f;
 #pragma unroll 4
             for (int i = l; i < end; i += share) {
                 const float2 v = channel(c0 + i);
@@ -816,19 +788,19 @@ __device__ __forceinline__ void group_records(const NormAct &p, int share, int64
             a = sum(a), b = sum(b);
             if (g < p.G && l == 0) to[g] = {a, b};
         } else {   // the mean about the first channel's, then squares about it
-            const float k = channel(c0).x, from = base(c0);
+            const double k = channel(c0).x;
+            double a = 0.0, b = 0.0;
 #pragma unroll 4
-            for (int i = l; i < end; i += share) a += (base(c0 + i) - from) + (channel(c0 + i).x - k);
-            const float off = sum(a) / (float)p.W;
+            for (int i = l; i < end; i += share) a += channel(c0 + i).x - k;
+            const double mean = k + sum(a) * inverse;
 #pragma unroll 4
             for (int i = l; i < end; i += share) {
-                const float2 v = channel(c0 + i);
-                const float d = ((base(c0 + i) - from) + (v.x - k)) - off;
-                b += v.y + (float)n * d * d;
+                const double2 v = channel(c0 + i);
+                const double d = v.x - mean;
+                b += fma((double)n * d, d, v.y);
             }
             b = sum(b);
-            const double mean = ((double)from + k) + off;
-            if (g < p.G && l == 0) to[g] = {(float)mean, (float)(mean - (double)(float)mean), b, 0.f};
+            if (g < p.G && l == 0) to[g] = {mean, b};
         }
     }
 }
@@ -890,25 +862,28 @@ __device__ __noinline__ void affine_gradients(const NormAct &p, int tile, double
 }
 
 // ------------------------------------------------------------ the kernel ----
+// Pairs of 32 bits that folding takes (at least what affine_gradients does).
+template <int VN, bool BACKWARD>
+__host__ __device__ constexpr int fold_entries() { return (BACKWARD ? (VN < 2 ? 2 : VN) : 2 * VN) * NA_THREADS; }
 template <int VN, bool BACKWARD>
 size_t shared_bytes(int C) {
     const Columns l(C, VN, 0);
-    return (size_t)std::max(VN, 2) * NA_THREADS * sizeof(float2) + (size_t)(BACKWARD ? 8 : 3) * l.cols * VN * sizeof(float) +
-           NA_THREADS * sizeof(float4) + (size_t)(l.cols * VN + 1) * sizeof(Stats);
+    return (size_t)fold_entries<VN, BACKWARD>() * sizeof(float2) + (size_t)(BACKWARD ? 8 : 3) * l.cols * VN * sizeof(float) +
+           NA_THREADS * sizeof(double2) + (size_t)(l.cols * VN + 1) * sizeof(Stats);
 }
 
 // ACT, DROP = -1: as the arguments say; DROP = 0: none, 1: the seed is in the arguments, 2: on the device.
 template <typename T, int VN, int ACT, int DROP, bool BACKWARD>
-__global__ void __launch_bounds__(NA_THREADS, BACKWARD ? 3 : 4) na_kernel(const __grid_constant__ NormAct p) {
+__global__ void __launch_bounds__(NA_THREADS, NA_BLOCKS) na_kernel(const __grid_constant__ NormAct p) {
     start_after_previous();
     extern __shared__ __align__(128) char shared[];
     __shared__ int next, told;
     float2 *fold = reinterpret_cast<float2 *>(shared);   // sums of threads, or records that are merged
     const Columns l(p.C, VN, threadIdx.x);
     Constants<VN, BACKWARD> k_sums, k_apply;
-    k_apply.at = reinterpret_cast<float *>(fold + (VN < 2 ? 2 : VN) * NA_THREADS);
+    k_apply.at = reinterpret_cast<float *>(fold + fold_entries<VN, BACKWARD>());
     k_sums.at = k_apply.at + 5 * l.cols * VN;
-    k_apply.scratch = reinterpret_cast<float4 *>(k_apply.at + ((BACKWARD ? 8 : 3) * l.cols * VN + 3) / 4 * 4);
+    k_apply.scratch = reinterpret_cast<double2 *>(k_apply.at + ((BACKWARD ? 8 : 3) * l.cols * VN + 3) / 4 * 4);
     k_apply.stats = reinterpret_cast<Stats *>(k_apply.scratch + NA_THREADS);
     const Philox<DROP != 1> rng(p.drop);
     const int tiles = BACKWARD && p.dweight ? (p.C + AFFINE_CHANNELS - 1) / AFFINE_CHANNELS : 0;
@@ -931,10 +906,12 @@ __global__ void __launch_bounds__(NA_THREADS, BACKWARD ? 3 : 4) na_kernel(const 
             if (hi <= lo) continue;   // a sample without rows
             if (sums) {
                 if constexpr (BACKWARD) bwd_sums_piece<T, VN, ACT, DROP>(p, l, rng, k_sums, chunk + s, s, lo, (int)(hi - lo), fold);
-                else stats_piece<T, VN>(p, l, chunk + s, lo, (int)(hi - lo), fold);
+                else stats_piece<T, VN>(p, l, lo, (int)(hi - lo), reinterpret_cast<double2 *>(fold));
                 sync_workers();
-                const float2 *channels = p.rec + (chunk + s) * p.C;   // (what this block has written)
-                group_records<BACKWARD, BlockTeam>(p, lanes_of_group<BlockTeam>(p), chunk + s, (int)(hi - lo), [&](int c) { return __ldcg(channels + c); }, [](int) { return 0.f; });
+                group_records<BACKWARD, BlockTeam>(p, lanes_of_group<BlockTeam>(p), chunk + s, (int)(hi - lo), [&](int c) {   // (what this block has written)
+                    if constexpr (BACKWARD) return __ldcg(p.rec + (chunk + s) * p.C + c);
+                    else return __ldcg(p.scratch + (int64_t)blockIdx.x * p.C + c);
+                });
                 count_piece<BACKWARD, BlockTeam>(p, p.spans[s], chunk, s, &told);
             } else {
                 bool there;
@@ -965,8 +942,7 @@ __global__ void __launch_bounds__(NA_THREADS, BACKWARD ? 3 : 4) na_kernel(const 
 enum { TILE_SUMS = 0, TILE_APPLY = 1, TILE_AFFINE = 2, TILE_END = 3, TILE_NONE = 4 };
 constexpr int RING_CHANNELS = 1024;                // of a row, at most (their constants take room from the ring)
 constexpr int RING_STAGES = 8;                     // at most
-constexpr int FOLD_SLOTS = 2;                      // pieces on their way to the clerk
-constexpr int FOLD_STRIDE = NA_THREADS + 2;        // of a channel of the lumps (two more: without bank conflicts)
+constexpr int FOLD_SLOTS = 2;                      // pieces on their way to the clerk, at most
 constexpr int RING_THREADS = NA_THREADS + 64;
 constexpr int RING_BLOCKS = 2;                     // on a multiprocessor
 struct __align__(16) Tile {
@@ -984,24 +960,39 @@ struct Ring {
     Piece pieces[FOLD_SLOTS];
     int told, abort;
 };
-// (behind the ring's tiles) two slots of sums, what is taken off the channels' values for each, constants
+// Whether whole rows of columns make a warp (64 channels: 8 columns, 4 rows): its lanes are then folded before the clerk has them.
+__host__ __device__ __forceinline__ bool warps_fold(const Columns &l) { return l.cols < 32 && 32 % l.cols == 0; }
+// Where sums of pieces wait for the clerk: 33 KB.  Backward pairs of 32 bits in two slots, forward of 64 in two where warps fold their own
+// (128 of them or fewer for each channel of the lumps), and in one otherwise.
+template <bool BACKWARD>
+struct Folds {
+    using Two = std::conditional_t<BACKWARD, float2, double2>;
+    static constexpr int BYTES = 2 * 8 * (NA_THREADS + 2) * (int)sizeof(float2);
+    int rows, stride, slots;   // rows of columns; from a channel of the lumps to the next, so that the clerk finds no bank conflicts
+    __device__ __forceinline__ explicit Folds(const Columns &l) {
+        rows = warps_fold(l) ? NA_THREADS / 32 : l.lanes;
+        stride = BACKWARD ? NA_THREADS + 2 : rows * l.cols | 1;
+        slots = BACKWARD || stride <= NA_THREADS / 2 + 1 ? FOLD_SLOTS : 1;
+    }
+};
+// (behind the ring's tiles) slots of sums, what is taken off the channels' values for each, constants
 struct RingMemory {
     char *stages;
-    float2 *fold;
+    char *fold;
     float *firsts, *constants;
     Stats *stats;
-    float4 *scratch;
+    double2 *scratch;
     __device__ __forceinline__ RingMemory(const NormAct &p, char *shared) {
         stages = shared;
-        fold = reinterpret_cast<float2 *>(shared + (size_t)p.stages * p.stage_bytes);
-        scratch = reinterpret_cast<float4 *>(fold + FOLD_SLOTS * 8 * FOLD_STRIDE);
+        fold = shared + (size_t)p.stages * p.stage_bytes;
+        scratch = reinterpret_cast<double2 *>(fold + Folds<true>::BYTES);
         stats = reinterpret_cast<Stats *>(scratch + NA_THREADS);
         constants = reinterpret_cast<float *>(stats + p.G);
         firsts = constants + 3 * p.V;   // (forward alone)
     }
 };
 inline size_t ring_bytes(int V, int G, bool backward) {   // without the tiles
-    return (size_t)FOLD_SLOTS * 8 * FOLD_STRIDE * sizeof(float2) + NA_THREADS * sizeof(float4) + (size_t)G * sizeof(Stats) + (size_t)(backward ? 8 : 3 + FOLD_SLOTS) * V * sizeof(float);
+    return (size_t)Folds<true>::BYTES + NA_THREADS * sizeof(double2) + (size_t)G * sizeof(Stats) + (size_t)(backward ? 8 : 3 + FOLD_SLOTS) * V * sizeof(float);
 }
 
 __device__ __forceinline__ void bulk_copy(uint32_t to, const void *from, uint32_t bytes, uint32_t bar, uint64_t policy) {
@@ -1112,57 +1103,54 @@ __device__ __forceinline__ void ring_producer(const NormAct &p, Ring &ring, cons
     }
 }
 
-// Whether whole rows of columns make a warp (64 channels: 8 columns, 4 rows): its lanes are then folded before the clerk has them.
-__device__ __forceinline__ bool warps_fold(const Columns &l) { return l.cols < 32 && 32 % l.cols == 0; }
-
 // Folds the sums of pieces over the row lanes and takes them from there.
 template <bool BACKWARD, bool PHASES>
 __device__ __forceinline__ void ring_clerk(const NormAct &p, Ring &ring, const RingMemory &m) {
     const int lane = threadIdx.x & 31;
     const Columns l(p.V, 8, 0);
-    const int lanes = warps_fold(l) ? NA_THREADS / 32 : l.lanes;
-    const bool few = !PHASES && lanes <= 8;   // one chain (with eight, a call of 942 points and 256 channels takes a microsecond more)
-    int parts = 1;                            // lanes of a channel
+    const Folds<BACKWARD> folds(l);
+    using Two = typename Folds<BACKWARD>::Two;
+    const bool few = !PHASES && folds.rows <= 8;   // one chain (with eight, a call of 942 points and 256 channels takes a microsecond more)
+    int parts = 1;                                 // lanes of a channel
     while (!few && 2 * parts * p.C <= 32) parts *= 2;
     const int share = lanes_of_group<WarpTeam>(p);
     Place slot;
     for (;;) {
-        slot.next(FOLD_SLOTS);
+        slot.next(folds.slots);
         if (!__all_sync(0xffffffffu, tc::mbar_wait_abortable(tc::smem_u32(&ring.folded[slot.at]), slot.parity, NA_STATUS, p.status, &ring.abort))) return;
         const Piece piece = ring.pieces[slot.at];
         if (piece.kind == TILE_END) return;
-        float2 *fold = m.fold + slot.at * 8 * FOLD_STRIDE;
+        Two *fold = reinterpret_cast<Two *>(m.fold) + slot.at * 8 * folds.stride;
         const float *firsts = m.firsts + slot.at * p.V;
         const int64_t number = piece.chunk + (int64_t)piece.s;
+        const double inverse = 1.0 / piece.rows;
         for (int base = 0; base < p.C; base += 32 / parts) {   // (the same rounds for all lanes)
             const int c = base + lane / parts;
-            float2 sums = make_float2(0.f, 0.f);
+            Two sums{};
             if (few) {
                 if (c >= p.C) continue;
-                const float2 *from = fold + c % 8 * FOLD_STRIDE + c / 8;
+                const Two *from = fold + c % 8 * folds.stride + c / 8;
 #pragma unroll
                 for (int q = 0; q < 8; ++q)
-                    if (q < lanes) sums = add2(sums, from[q * l.cols]);
+                    if (q < folds.rows) sums.x += from[q * l.cols].x, sums.y += from[q * l.cols].y;
             } else {
-                Chains chains;
+                Chains<Two> chains;
                 if (c < p.C)
-                    for (int at = c; at < (PHASES ? p.V : c + 1); at += p.C) chains.add(fold + at % 8 * FOLD_STRIDE + at / 8, lane % parts, parts, lanes, l.cols);
+                    for (int at = c; at < (PHASES ? p.V : c + 1); at += p.C) chains.add(fold + at % 8 * folds.stride + at / 8, lane % parts, parts, folds.rows, l.cols);
                 sums = chains.sum();
             }
-            for (int o = parts / 2; o > 0; o >>= 1) sums = add2(sums, make_float2(__shfl_xor_sync(0xffffffffu, sums.x, o), __shfl_xor_sync(0xffffffffu, sums.y, o)));
+            for (int o = parts / 2; o > 0; o >>= 1) sums.x += __shfl_xor_sync(0xffffffffu, sums.x, o), sums.y += __shfl_xor_sync(0xffffffffu, sums.y, o);
             if (c >= p.C || lane % parts) continue;
-            float a = sums.x, b = sums.y;
             if constexpr (BACKWARD) {
-                b *= (float)__ldg(p.rstd + (int64_t)piece.s * p.G + group_of(p, c));
-                if (p.dweight) p.rec[number * p.C + c] = make_float2(a, b);
+                sums.y *= (float)__ldg(p.rstd + (int64_t)piece.s * p.G + group_of(p, c));
+                if (p.dweight) p.rec[number * p.C + c] = sums;
             } else {
-                const float off = a / (float)piece.rows;   // (not by a rounded inverse: its error is the same in every piece)
-                b = fmaxf(b - a * off, 0.f), a = off;
+                sums = moments_of(firsts[c], sums.x, sums.y, inverse);
             }
-            fold[c % 8 * FOLD_STRIDE + c / 8] = make_float2(a, b);
+            fold[c % 8 * folds.stride + c / 8] = sums;
         }
         __syncwarp();
-        group_records<BACKWARD, WarpTeam>(p, share, number, piece.rows, [&](int c) { return fold[c % 8 * FOLD_STRIDE + c / 8]; }, [&](int c) { return firsts[c]; });
+        group_records<BACKWARD, WarpTeam>(p, share, number, piece.rows, [&](int c) { return fold[c % 8 * folds.stride + c / 8]; });
         __syncwarp();
         if (lane == 0) tc::mbar_arrive(tc::smem_u32(&ring.taken[slot.at]));
         count_piece<BACKWARD, WarpTeam>(p, p.spans[piece.s], piece.chunk, piece.s, &ring.told);
@@ -1218,6 +1206,8 @@ template <typename T, int ACT, int DROP, bool BACKWARD, bool PHASES>
 __device__ __forceinline__ void ring_worker(const NormAct &p, Ring &ring, const RingMemory &m) {
     constexpr int VN = 8, P = 4, UNROLL = BACKWARD && DROP ? 1 : 2;   // (more spills registers)
     const Columns l(p.V, VN, threadIdx.x);
+    const Folds<BACKWARD> folds(l);
+    using Two = typename Folds<BACKWARD>::Two;
     const Philox<DROP != 1> rng(p.drop);
     const bool mine = l.lane < l.lanes;
     const int c0 = l.col * VN, step = l.lanes * p.V;   // elements from one of a thread's rows to its next
@@ -1250,92 +1240,65 @@ __device__ __forceinline__ void ring_worker(const NormAct &p, Ring &ring, const 
     const auto rows_at = [&] { return reinterpret_cast<const T *>(m.stages + (size_t)place.at * p.stage_bytes) + c0; };
     // A slot for sums; false: the clerk has not come for the ones before.
     const auto next_slot = [&]() -> bool {
-        slot.next(FOLD_SLOTS);
-        return ++pieces <= FOLD_SLOTS || __all_sync(0xffffffffu, tc::mbar_wait(tc::smem_u32(&ring.taken[slot.at]), slot.parity ^ 1, NA_STATUS, p.status));
+        slot.next(folds.slots);
+        return ++pieces <= folds.slots || __all_sync(0xffffffffu, tc::mbar_wait(tc::smem_u32(&ring.taken[slot.at]), slot.parity ^ 1, NA_STATUS, p.status));
     };
     const auto send = [&](const Piece &piece) {
         if (threadIdx.x == 0) ring.pieces[slot.at] = piece;
         __syncwarp();
         if ((threadIdx.x & 31) == 0) tc::mbar_arrive(tc::smem_u32(&ring.folded[slot.at]));
     };
+    // A piece's sums, `part(i)` those of the lump's channels, into its slot: over the warp's row lanes first, where that is whole.
+    const auto fold_and_send = [&](const Piece &piece, auto part) {
+        Two sums[VN];
+#pragma unroll
+        for (int i = 0; i < VN; ++i) {
+            sums[i] = part(i);
+            if (warps_fold(l))
+                for (int o = 16; o >= l.cols; o >>= 1) sums[i].x += __shfl_xor_sync(0xffffffffu, sums[i].x, o), sums[i].y += __shfl_xor_sync(0xffffffffu, sums[i].y, o);
+        }
+        if (warps_fold(l) ? (threadIdx.x & 31) < l.cols : mine) {
+            Two *fold = reinterpret_cast<Two *>(m.fold) + slot.at * 8 * folds.stride + (warps_fold(l) ? (threadIdx.x >> 5) * l.cols + (threadIdx.x & 31) : threadIdx.x);
+#pragma unroll
+            for (int i = 0; i < VN; ++i) fold[i * folds.stride] = sums[i];
+        }
+        send(piece);
+    };
     next_tile();
     for (;;) {
-        if (t.kind == TILE_SUMS) {
-            float2 a[P], b[P], k[P], fa[P], fb[P];   // k: what is taken off x
+        if (t.kind == TILE_SUMS && !BACKWARD) {
             const int s = t.s, chunk = t.chunk;
-            int64_t unsettled = -1;   // a lump with a ReLU's argument next to its border (of two in a thread's part of a piece, the last)
-            if (BACKWARD && k_sums.s != s) {
-                if (!sync_workers_and(true)) break;
-                k_sums.template load<PHASES>(p, l, s, 0, false);
-            }
             const bool free = next_slot();
+            Lump<T, VN> k;
+            if constexpr (PHASES) {
+                const T *first = rows_at() - c0 + ends().x;
+                int c = channel_of(p, c0);
 #pragma unroll
-            for (int j = 0; j < P; ++j) a[j] = b[j] = both(0.f);
-            if constexpr (BACKWARD) {
-                k_sums.read_all(l, K_MU, k), k_sums.read_all(l, K_A, fa), k_sums.read_all(l, K_B, fb);
+                for (int i = 0; i < VN; ++i) {
+                    k.set(i, to_f32<T>(first[c]));
+                    if (++c == p.C) c = 0;
+                }
             } else {
-                if constexpr (PHASES) {
-                    const int2 e = ends();
-                    const T *tile = rows_at() - c0 + e.x;
-                    const int n = (e.y - e.x) / p.C, m = min(n, SHIFT_ROWS), first = channel_of(p, c0);
-                    minus_shift<T, VN>(m, k, [&](int row) {
-                        Lump<T, VN> v;
-                        const T *from = tile + row * n / m * p.C;
-                        int c = first;
-#pragma unroll
-                        for (int i = 0; i < VN; ++i) {
-                            v.set(i, to_f32<T>(from[c]));
-                            if (++c == p.C) c = 0;
-                        }
-                        return v;
-                    });
-                } else {
-                    const int m = min(t.n, SHIFT_ROWS);
-                    minus_shift<T, VN>(m, k, [&](int row) {
-                        Lump<T, VN> v;
-                        v.load(rows_at() + row * t.n / m * p.V);
-                        return v;
-                    });
-                }
-                if (l.lane == 0 && free) {   // (C of V are read)
-#pragma unroll
-                    for (int j = 0; j < P; ++j) *reinterpret_cast<float2 *>(m.firsts + slot.at * p.V + c0 + 2 * j) = neg2(k[j]);
-                }
+                k.load(rows_at());
             }
+            if (l.lane == 0 && free) {   // (C of V are read)
+#pragma unroll
+                for (int i = 0; i < VN; ++i) m.firsts[slot.at * p.V + c0 + i] = k.get(i);
+            }
+            Moments<VN> sums(k);
             int rows = 0;
             for (bool more = true; more;) {
                 const T *x = rows_at();
                 if (mine)
-#pragma unroll UNROLL
+#pragma unroll 2
                     for (int r = l.lane, at = l.lane * p.V; r < t.n; r += l.lanes, at += step) {
-                        BackwardRows<T, VN, ACT, DROP, 1> in;
-                        in.x.v[0].load(x + at);
-                        if constexpr (BACKWARD) {
-                            in.g.v[0].load(x + tensor + at);
-                            if (p.residual) in.res.v[0].load(x + 2 * tensor + at);
-                            if (DROP) rng.template words<VN>((uint64_t)(t.from + at + c0), in.words[0]);
-                        }
-                        float2 xc[P], gz[P];
-                        if constexpr (BACKWARD)
-                            if (in.template gz<P, ACT == ACT_RELU ? BORDER_TOLD : BORDER_AS_IT_IS>(p, s, c0, 0, 0, k, fa, fb, xc, gz)) unsettled = t.from + at + c0;
-                        if constexpr (!BACKWARD)
-#pragma unroll
-                            for (int j = 0; j < P; ++j) xc[j] = add2(pair_of(in.x.v[0], j), k[j]);
+                        Lump<T, VN> v;
+                        v.load(x + at);
                         if (PHASES && cut(at + c0)) {
                             const int2 e = ends();
-#pragma unroll
-                            for (int j = 0; j < P; ++j) {
-                                xc[j] = within(xc[j], at + c0 + 2 * j, e.x, e.y);
-                                if (BACKWARD) gz[j] = within(gz[j], at + c0 + 2 * j, e.x, e.y);
-                            }
-                        }
-#pragma unroll
-                        for (int j = 0; j < P; ++j) {
-                            if constexpr (BACKWARD) {
-                                a[j] = add2(a[j], gz[j]), b[j] = fma2(gz[j], xc[j], b[j]);
-                            } else {
-                                a[j] = add2(a[j], xc[j]), b[j] = fma2(xc[j], xc[j], b[j]);
-                            }
+                            sums.add(v, e.x - at - c0, e.y - at - c0);
+                        } else {
+                            sums.add(v);
                         }
                     }
                 rows = t.last;
@@ -1345,7 +1308,49 @@ __device__ __forceinline__ void ring_worker(const NormAct &p, Ring &ring, const 
                 if (t.kind == TILE_NONE) more = false;
             }
             if (!free) t.kind = TILE_NONE;
-            if constexpr (BACKWARD && ACT == ACT_RELU) {
+            if constexpr (!BACKWARD)
+                if (t.kind != TILE_NONE) fold_and_send(Piece{TILE_SUMS, s, chunk, rows}, [&](int i) { return make_double2(sums.a[i], sums.b[i]); });
+        } else if (t.kind == TILE_SUMS) {
+            float2 a[P], b[P], mu[P], fa[P], fb[P];
+            const int s = t.s, chunk = t.chunk;
+            int64_t unsettled = -1;   // a lump with a ReLU's argument next to its border (of two in a thread's part of a piece, the last)
+            if (k_sums.s != s) {
+                if (!sync_workers_and(true)) break;
+                k_sums.template load<PHASES>(p, l, s, 0, false);
+            }
+            const bool free = next_slot();
+#pragma unroll
+            for (int j = 0; j < P; ++j) a[j] = b[j] = both(0.f);
+            k_sums.read_all(l, K_MU, mu), k_sums.read_all(l, K_A, fa), k_sums.read_all(l, K_B, fb);
+            int rows = 0;
+            for (bool more = true; more;) {
+                const T *x = rows_at();
+                if (mine)
+#pragma unroll UNROLL
+                    for (int r = l.lane, at = l.lane * p.V; r < t.n; r += l.lanes, at += step) {
+                        BackwardRows<T, VN, ACT, DROP, 1> in;
+                        in.x.v[0].load(x + at);
+                        in.g.v[0].load(x + tensor + at);
+                        if (p.residual) in.res.v[0].load(x + 2 * tensor + at);
+                        if (DROP) rng.template words<VN>((uint64_t)(t.from + at + c0), in.words[0]);
+                        float2 xc[P], gz[P];
+                        if (in.template gz<P, ACT == ACT_RELU ? BORDER_TOLD : BORDER_AS_IT_IS>(p, s, c0, 0, 0, mu, fa, fb, xc, gz)) unsettled = t.from + at + c0;
+                        if (PHASES && cut(at + c0)) {
+                            const int2 e = ends();
+#pragma unroll
+                            for (int j = 0; j < P; ++j) xc[j] = within(xc[j], at + c0 + 2 * j, e.x, e.y), gz[j] = within(gz[j], at + c0 + 2 * j, e.x, e.y);
+                        }
+#pragma unroll
+                        for (int j = 0; j < P; ++j) a[j] = add2(a[j], gz[j]), b[j] = fma2(gz[j], xc[j], b[j]);
+                    }
+                rows = t.last;
+                more = !rows;
+                release();
+                next_tile();
+                if (t.kind == TILE_NONE) more = false;
+            }
+            if (!free) t.kind = TILE_NONE;
+            if constexpr (ACT == ACT_RELU) {
                 if (unsettled >= 0) {
                     TwoSums sums;
 #pragma unroll
@@ -1356,22 +1361,9 @@ __device__ __forceinline__ void ring_worker(const NormAct &p, Ring &ring, const 
                 }
                 __syncwarp();
             }
-            if (t.kind != TILE_NONE) {
-                if (warps_fold(l)) {   // over the warp's row lanes first
-                    for (int o = 16; o >= l.cols; o >>= 1)
-#pragma unroll
-                        for (int j = 0; j < P; ++j) {
-                            a[j] = add2(a[j], make_float2(__shfl_xor_sync(0xffffffffu, a[j].x, o), __shfl_xor_sync(0xffffffffu, a[j].y, o)));
-                            b[j] = add2(b[j], make_float2(__shfl_xor_sync(0xffffffffu, b[j].x, o), __shfl_xor_sync(0xffffffffu, b[j].y, o)));
-                        }
-                }
-                if (!warps_fold(l) || (threadIdx.x & 31) < l.cols) {
-                    float2 *fold = m.fold + slot.at * 8 * FOLD_STRIDE + (warps_fold(l) ? (threadIdx.x >> 5) * l.cols + (threadIdx.x & 31) : threadIdx.x);
-#pragma unroll
-                    for (int i = 0; i < VN; ++i) fold[i * FOLD_STRIDE] = i % 2 ? make_float2(a[i / 2].y, b[i / 2].y) : make_float2(a[i / 2].x, b[i / 2].x);
-                }
-                send(Piece{TILE_SUMS, s, chunk, rows});
-            }
+            if constexpr (BACKWARD)
+                if (t.kind != TILE_NONE)
+                    fold_and_send(Piece{TILE_SUMS, s, chunk, rows}, [&](int i) { return i % 2 ? make_float2(a[i / 2].y, b[i / 2].y) : make_float2(a[i / 2].x, b[i / 2].x); });
         } else if (t.kind == TILE_APPLY) {
             const int s = t.s;
             if (k_apply.s != s) {
@@ -1480,7 +1472,7 @@ int run_kernel(const NormAct &p, cudaStream_t stream) {
     if (smem > 40 << 10)
         if (int rc = allow_shared_memory((const void *)kernel, &allowed)) return rc;
     const int64_t tickets = 2 * (int64_t)p.chunks + (BACKWARD && p.dweight ? (p.C + AFFINE_CHANNELS - 1) / AFFINE_CHANNELS : 0);
-    launch_after(kernel, (unsigned)std::min<int64_t>(tickets, (BACKWARD ? 3 : 4) * num_sms()), NA_THREADS, smem, stream, p);
+    launch_after(kernel, (unsigned)std::min<int64_t>(tickets, NA_BLOCKS * num_sms()), NA_THREADS, smem, stream, p);
     PCX_LAUNCH_CHECK();
     return PCX_OK;
 }
