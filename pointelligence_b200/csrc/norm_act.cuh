@@ -352,9 +352,17 @@ __device__ __forceinline__ bool wait_for(const int *word, int value, unsigned in
 
 // What the rows of a sample are mapped by, per channel of a pass, in shared memory: floats k of a lump's quad h lie side by side over the
 // columns, so that a warp reads them without conflicts.  (In registers they were most of what a thread held: 24 to 40 floats.)
-// Forward z = x a + b, with the mean in b: that rounds z by 2^-24 of |mean| / deviation more, as the mean's own rounding does.  Backward
-// z = (x - mu) a + b, as sums of gz (x - mu) want the difference, and dx = gz a - m1 - (x - mu) m2.
+// z = (x - mu) a + b in both directions: mu is the mean rounded to 32 bits, and what that leaves of it is in b.  So z is off by roundings of its
+// own terms, however many deviations the mean is from zero.  (With the mean in b whole, z = x a + b rounds by 2^-24 of |mean| / deviation.)
+// Backward dx = gz a + m1 + (x - mu) m2, where m1 has the mean's rest too.
 enum { K_A = 0, K_B = 1, K_MU = 2, K_M1 = 3, K_M2 = 4 };
+struct Mapping {
+    float a, b, mu, rest;
+    __device__ __forceinline__ Mapping(double mean, double rstd, float w, float bias) {
+        mu = (float)mean, a = (float)(rstd * w), rest = (float)(mean - mu);
+        b = (float)fma(-(mean - mu), (double)a, (double)bias);
+    }
+};
 template <int VN, bool BACKWARD>
 struct Constants {
     static constexpr int QUAD = VN < 4 ? VN : 4, PAIRS = QUAD < 2 ? 1 : QUAD / 2, QUADS = VN / QUAD;
@@ -383,10 +391,11 @@ struct Constants {
     template <bool PHASES = false>
     __device__ __forceinline__ bool load(const NormAct &p, const Columns &l, int64_t s_, int pass_, bool second) {
         const int c0 = pass_ * l.cols * VN, c1 = min(p.C, c0 + l.cols * VN), g0 = group_of(p, c0);
-        float w = 1.f, bias = 0.f, mu = 0.f, rs = 0.f;   // of the thread's first channel: read before the wait
+        float w = 1.f, bias = 0.f;   // of the thread's first channel: read before the wait
+        double mean = 0.0, rstd = 0.0;
         const auto known = [&](int c) {
             if (p.weight) w = __ldg(p.weight + c), bias = __ldg(p.bias + c);
-            if (BACKWARD) mu = (float)__ldg(p.mean + s_ * p.G + group_of(p, c)), rs = (float)__ldg(p.rstd + s_ * p.G + group_of(p, c));
+            if (BACKWARD) mean = __ldg(p.mean + s_ * p.G + group_of(p, c)), rstd = __ldg(p.rstd + s_ * p.G + group_of(p, c));
         };
         if (c0 + (int)threadIdx.x < c1) known(c0 + threadIdx.x);
         if (second) {
@@ -402,13 +411,13 @@ struct Constants {
             if (t >= NA_THREADS) known(c0 + t);
             Stats m = {};
             if (second) m = stats[group_of(p, c0 + t) - g0];
-            if (!BACKWARD) mu = (float)m.x, rs = (float)m.y;
-            const float b = BACKWARD ? bias : (float)fma(-(double)m.x, (double)m.y * w, (double)bias);
+            if (!BACKWARD) mean = m.x, rstd = m.y;
+            const Mapping map(mean, rstd, w, bias);
+            const float m2 = (float)(-m.y * rstd * rstd), m1 = (float)(-m.x * rstd) - map.rest * m2;
             for (int v = t; v < (PHASES ? p.V : t + 1); v += p.C) {
                 float *to = at + ((v % VN / QUAD) * l.cols + v / VN) * QUAD + v % QUAD;
-                to[K_A * stride] = rs * w, to[K_B * stride] = b;
-                if (BACKWARD) to[K_MU * stride] = -mu;
-                if (BACKWARD && second) to[K_M1 * stride] = (float)-m.x * rs, to[K_M2 * stride] = (float)-m.y * rs * rs;
+                to[K_A * stride] = map.a, to[K_B * stride] = map.b, to[K_MU * stride] = -map.mu;
+                if (BACKWARD && second) to[K_M1 * stride] = m1, to[K_M2 * stride] = m2;
             }
         }
         sync_workers();
@@ -566,14 +575,14 @@ __device__ __forceinline__ bool apply_piece(const NormAct &p, const Columns &l, 
             }
 #pragma unroll
             for (int h = 0; h < Constants<VN, false>::QUADS; ++h) {
-                float2 a[PAIRS], b[PAIRS];
-                k.read(l, K_A, h, a), k.read(l, K_B, h, b);
+                float2 mu[PAIRS], a[PAIRS], b[PAIRS];
+                k.read(l, K_MU, h, mu), k.read(l, K_A, h, a), k.read(l, K_B, h, b);
 #pragma unroll
                 for (int u = 0; u < U; ++u)
 #pragma unroll
                     for (int i = 0; i < PAIRS; ++i) {
                         const int j = h * PAIRS + i;
-                        float2 z = fma2(pair_of(v.v[u], j), a[i], b[i]);
+                        float2 z = fma2(add2(pair_of(v.v[u], j), mu[i]), a[i], b[i]);
                         if (res) z = add2(z, pair_of(q.v[u], j));
                         z = act2(act, z);
                         if (drop) z = drop2<VN>(p, words[u], j, z);
@@ -591,6 +600,12 @@ __device__ __forceinline__ bool apply_piece(const NormAct &p, const Columns &l, 
 }
 
 // ------------------------------------------------------------ backward ----
+// Sums of gz and gz * xh of a channel, from sums of gz and gz (x - mu).
+__device__ __forceinline__ float2 sums_of(const NormAct &p, int64_t s, int c, float a, float b) {
+    const double mean = __ldg(p.mean + s * p.G + group_of(p, c));
+    return make_float2(a, fmaf(-(float)(mean - (float)mean), a, b) * (float)__ldg(p.rstd + s * p.G + group_of(p, c)));
+}
+
 // The ReLU's argument where 32 bits do not settle its sign: in fp64 it is the definition's.  That is asked for where the argument is this
 // small a part of what it is made of (its roundings are some 2^-23 of that), and for the sums alone: a sign that comes out on the
 // other side moves one element of the gradients of x and the residual, but a sum over a million rows by a whole gradient.
@@ -684,7 +699,7 @@ __device__ __forceinline__ void bwd_sums_piece(const NormAct &p, const Columns &
             in.load(p, l, from, r + U * l.lanes, n);
         }
         fold_lanes<VN>(l, pass, fold, [&](int i) { return i % 2 ? make_float2(a[i / 2].y, b[i / 2].y) : make_float2(a[i / 2].x, b[i / 2].x); }, [&](int c, float sa, float sb) {
-            p.rec[piece * p.C + c] = make_float2(sa, sb * (float)__ldg(p.rstd + s * p.G + group_of(p, c)));
+            p.rec[piece * p.C + c] = sums_of(p, s, c, sa, sb);
         });
     }
 }
@@ -1142,7 +1157,7 @@ __device__ __forceinline__ void ring_clerk(const NormAct &p, Ring &ring, const R
             for (int o = parts / 2; o > 0; o >>= 1) sums.x += __shfl_xor_sync(0xffffffffu, sums.x, o), sums.y += __shfl_xor_sync(0xffffffffu, sums.y, o);
             if (c >= p.C || lane % parts) continue;
             if constexpr (BACKWARD) {
-                sums.y *= (float)__ldg(p.rstd + (int64_t)piece.s * p.G + group_of(p, c));
+                sums = sums_of(p, piece.s, c, sums.x, sums.y);
                 if (p.dweight) p.rec[number * p.C + c] = sums;
             } else {
                 sums = moments_of(firsts[c], sums.x, sums.y, inverse);
@@ -1187,7 +1202,8 @@ __device__ __noinline__ void settle_sums(const NormAct &p, int64_t from, int64_t
         for (int i = 0; i < 2; ++i) {   // (as Constants::load makes them)
             const int c = PHASES ? channel_of(p, c0 + 2 * j + i) : c0 + 2 * j + i;
             const int64_t g = s * p.G + group_of(p, c);
-            v[i] = -(float)__ldg(p.mean + g), v[2 + i] = (float)__ldg(p.rstd + g) * (p.weight ? __ldg(p.weight + c) : 1.f), v[4 + i] = p.weight ? __ldg(p.bias + c) : 0.f;
+            const Mapping map(__ldg(p.mean + g), __ldg(p.rstd + g), p.weight ? __ldg(p.weight + c) : 1.f, p.weight ? __ldg(p.bias + c) : 0.f);
+            v[i] = -map.mu, v[2 + i] = map.a, v[4 + i] = map.b;
         }
         mu[j] = make_float2(v[0], v[1]), a[j] = make_float2(v[2], v[3]), b[j] = make_float2(v[4], v[5]);
     }
@@ -1371,8 +1387,8 @@ __device__ __forceinline__ void ring_worker(const NormAct &p, Ring &ring, const 
                 if (!k_apply.template load<PHASES>(p, l, s, 0, true)) break;
             }
             float2 mu[P], fa[P], fb[P], m1[P], m2[P];
-            k_apply.read_all(l, K_A, fa), k_apply.read_all(l, K_B, fb);
-            if constexpr (BACKWARD) k_apply.read_all(l, K_MU, mu), k_apply.read_all(l, K_M1, m1), k_apply.read_all(l, K_M2, m2);
+            k_apply.read_all(l, K_MU, mu), k_apply.read_all(l, K_A, fa), k_apply.read_all(l, K_B, fb);
+            if constexpr (BACKWARD) k_apply.read_all(l, K_M1, m1), k_apply.read_all(l, K_M2, m2);
             do {
                 const T *x = rows_at();
                 if (!BACKWARD && t.last) k_apply.put_stats(p, l);
@@ -1393,7 +1409,7 @@ __device__ __forceinline__ void ring_worker(const NormAct &p, Ring &ring, const 
                                 set_pair(in.g.v[0], j, gz[j]);
                                 set_pair(in.x.v[0], j, fma2(gz[j], fa[j], fma2(xc[j], m2[j], m1[j])));
                             } else {
-                                float2 z = fma2(pair_of(in.x.v[0], j), fa[j], fb[j]);
+                                float2 z = fma2(add2(pair_of(in.x.v[0], j), mu[j]), fa[j], fb[j]);
                                 if (p.residual) z = add2(z, pair_of(in.res.v[0], j));
                                 z = act2(ACT, z);
                                 if (DROP) z = drop2<VN>(p, in.words[0], j, z);
