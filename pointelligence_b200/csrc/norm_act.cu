@@ -156,7 +156,7 @@ int run(const int64_t *d_lengths, NormAct &p, int dtype, int activation, std::in
         // (Where two tiles of 24 KB do not fit, smaller ones: 1024 channels, bf16, backward 292 us of 70 million elements, 458 by the general
         // kernel; where they do, three of two thirds are no better: 512 channels with a residual 230 and 252.)
         const int stage = room >= 2 * NA_STAGE_BYTES ? NA_STAGE_BYTES : room / 3;
-        p.tile_rows = lanes * std::max(1, stage / (lanes * row_bytes * tensors));
+        p.tile_rows = lanes * std::max(1, stage / (lanes * row_bytes * tensors));   // (at most 12 of a thread: lanes are more than half of the threads)
         p.sums_tile_rows = BACKWARD ? p.tile_rows : p.tile_rows * tensors;
         p.stage_bytes = (p.tile_rows * row_bytes * tensors + 127) / 128 * 128;
         p.stages = std::min(RING_STAGES, room / p.stage_bytes);

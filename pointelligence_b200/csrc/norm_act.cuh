@@ -208,6 +208,8 @@ __device__ __forceinline__ bool sync_workers_and(bool v) {
     return all != 0;
 }
 
+struct Stats { double x, y; };   // mean and rstd, or the backward's two means
+
 // Below zero, by roundings, is zero; a NaN stays one.
 __device__ __forceinline__ double not_below_zero(double v) { return v < 0.0 ? 0.0 : v; }
 
@@ -291,7 +293,6 @@ struct RecordSums<false> {
 // workers: mean and rstd, or the backward's two means.  Every block does this for itself, with the sample's windows counted: a block
 // that did it for all would keep them waiting for one more turn through the L2.  Threads stand side by side on the groups and, where
 // there are fewer of them, in rows on the records.
-struct Stats { double x, y; };
 template <bool BACKWARD>
 __device__ __forceinline__ void merge_groups(const NormAct &p, const Records<BACKWARD> &r, int groups, Stats *stats, double2 *scratch) {
     const int wide = min(groups, NA_THREADS), at = threadIdx.x % wide, q = threadIdx.x / wide;
@@ -546,6 +547,49 @@ __device__ __forceinline__ float2 drop2(const NormAct &p, const uint32_t *words,
     return make_float2((words[j] << 16) > p.drop.over ? v.x : 0.f, words[j] > p.drop.over ? v.y : 0.f);
 }
 
+// ------------------------------------------------------------ signs ----
+// In the backward pass a ReLU's argument z = (t = (x - mu) a + b) + residual has its sign from fp64 where 32 bits do not settle it: on the other
+// side, an element would have a whole gradient too much or too little, and so would dbias and dweight.  (Forward it matters to no more than
+// a rounding, and costs 6 us of 115 for 1.1 million rows of 64 channels.)  With u = 2^-24, z is off by u (2 |(x - mu) a| + |b| + |t| + |z|) at most, which for a z near zero, where
+// |t| is next to |residual| and |(x - mu) a| below |t| + |b|, is 3 u (|b| + |residual|): z is settled beyond 4 u of these.
+constexpr float NEAR_BORDER = 0x1p-22f;
+__device__ __forceinline__ float exact_argument(const NormAct &p, int64_t s, int c, float x, float residual) {
+    const int64_t g = s * p.G + group_of(p, c);
+    const double xh = ((double)x - __ldg(p.mean + g)) * __ldg(p.rstd + g);
+    return (float)((p.weight ? xh * __ldg(p.weight + c) + __ldg(p.bias + c) : xh) + residual);
+}
+// Settles a pair of arguments where they are next to the border.
+template <int VN>
+__device__ __forceinline__ void settle(const NormAct &p, int64_t s, int c, float2 x, float2 b, float2 residual, float2 &z) {
+    if (fabsf(z.x) < NEAR_BORDER * (fabsf(b.x) + fabsf(residual.x))) z.x = exact_argument(p, s, channel_of(p, c), x.x, residual.x);
+    if (VN > 1 && fabsf(z.y) < NEAR_BORDER * (fabsf(b.y) + fabsf(residual.y))) z.y = exact_argument(p, s, channel_of(p, c + 1), x.y, residual.y);
+}
+// Whether a ring's lump has such an argument, for the loops that all elements go through: its least one beside its largest offset (`b_most`: of
+// the thread's eight) and residual, and where that is near, one by one.  (Zeros of a channel without offset and residual are not near.)
+struct Least {
+    float z = INFINITY;
+    __device__ __forceinline__ void take(float2 v) { z = fminf(z, fminf(fabsf(v.x), fabsf(v.y))); }
+    // `residual(j)` of a pair; (a NaN in one channel: the others are looked at)
+    template <typename Residual>
+    __device__ __forceinline__ bool near(const float2 (&args)[4], const float2 *b, float b_most, float r_most, Residual residual) const {
+        if (z >= NEAR_BORDER * (b_most + r_most)) return false;
+        bool any = false;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float2 r = residual(j);
+            any |= fabsf(args[j].x) < NEAR_BORDER * (fabsf(b[j].x) + fabsf(r.x));
+            any |= fabsf(args[j].y) < NEAR_BORDER * (fabsf(b[j].y) + fabsf(r.y));
+        }
+        return any;
+    }
+};
+__device__ __forceinline__ float largest(const float2 (&v)[4]) {
+    float m = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) m = fmaxf(m, fmaxf(fabsf(v[j].x), fabsf(v[j].y)));
+    return m;
+}
+
 // ------------------------------------------------------------ second pass, forward ----
 template <typename T, int VN, int ACT, int DROP>
 __device__ __forceinline__ bool apply_piece(const NormAct &p, const Columns &l, const Philox<DROP != 1> &rng, Constants<VN, false> &k, int64_t s, int64_t lo, int n, bool owner) {
@@ -606,17 +650,6 @@ __device__ __forceinline__ float2 sums_of(const NormAct &p, int64_t s, int c, fl
     return make_float2(a, fmaf(-(float)(mean - (float)mean), a, b) * (float)__ldg(p.rstd + s * p.G + group_of(p, c)));
 }
 
-// The ReLU's argument where 32 bits do not settle its sign: in fp64 it is the definition's.  That is asked for where the argument is this
-// small a part of what it is made of (its roundings are some 2^-23 of that), and for the sums alone: a sign that comes out on the
-// other side moves one element of the gradients of x and the residual, but a sum over a million rows by a whole gradient.
-constexpr float NEAR_BORDER = 0x1p-20f;
-__device__ __noinline__ float exact_argument(const NormAct &p, int64_t s, int c, float x, float residual) {
-    const int64_t g = s * p.G + group_of(p, c);
-    const double xh = ((double)x - __ldg(p.mean + g)) * __ldg(p.rstd + g);
-    return (float)((p.weight ? xh * __ldg(p.weight + c) + __ldg(p.bias + c) : xh) + residual);
-}
-enum { BORDER_AS_IT_IS = 0, BORDER_TOLD = 1, BORDER_SETTLED = 2 };
-
 // Rows of what both passes of the backward read, and gz of a pair of them.
 template <typename T, int VN, int ACT, int DROP, int U>
 struct BackwardRows {
@@ -635,29 +668,45 @@ struct BackwardRows {
             for (int u = 0; u < U; ++u) rng.words<VN>((uint64_t)(from + (r + u * l.lanes) * p.C), words[u]);
         }
     }
-    // x - mean and gz of COUNT pairs from the j0-th on, of sample s, the lump's first channel c0.  The answer: a ReLU's argument is next to
-    // its border (BORDER_TOLD).
-    template <int COUNT, int BORDER>
-    __device__ __forceinline__ bool gz(const NormAct &p, int64_t s, int c0, int u, int j0, const float2 *mu, const float2 *a, const float2 *b, float2 *xc, float2 *out) const {
+    // gz of a ring's lump, and whether it is next to a ReLU's border (then all zeros, if such are to be left out).
+    template <bool LEFT_OUT>
+    __device__ __forceinline__ bool gz_told(const NormAct &p, float b_most, const float2 *mu, const float2 *a, const float2 *b, float2 *xc, float2 *out) {
+        float2 z[P];
+        Least least;
+#pragma unroll
+        for (int j = 0; j < P; ++j) {
+            xc[j] = add2(pair_of(x.v[0], j), mu[j]);
+            z[j] = fma2(xc[j], a[j], b[j]);
+            if (p.residual) z[j] = add2(z[j], pair_of(res.v[0], j));
+            least.take(z[j]);
+        }
+        const bool near = least.near(z, b, b_most, p.residual ? res.v[0].largest() : 0.f, [&](int j) { return p.residual ? pair_of(res.v[0], j) : both(0.f); });
+        if (LEFT_OUT) {
+#pragma unroll
+            for (int w = 0; w < Lump<T, VN>::WORDS; ++w) g.v[0].w[w] = near ? 0u : g.v[0].w[w];
+        }
+#pragma unroll
+        for (int j = 0; j < P; ++j) {
+            const float2 v = act2_backward(ACT_RELU, z[j], pair_of(g.v[0], j));
+            out[j] = DROP ? drop2<VN>(p, words[0], j, v) : v;
+        }
+        return near;
+    }
+    // x - mu and gz of COUNT pairs from the j0-th on, of sample s, the lump's first channel c0.
+    template <int COUNT, bool SETTLED>
+    __device__ __forceinline__ void gz(const NormAct &p, int64_t s, int c0, int u, int j0, const float2 *mu, const float2 *a, const float2 *b, float2 *xc, float2 *out) const {
         const int act = ACT < 0 ? p.act : ACT;
-        bool near = false;
 #pragma unroll
         for (int j = 0; j < COUNT; ++j) {
             const float2 xs = pair_of(x.v[u], j0 + j), rs = p.residual ? pair_of(res.v[u], j0 + j) : both(0.f);
             xc[j] = add2(xs, mu[j]);
             float2 z = fma2(xc[j], a[j], b[j]);
             if (p.residual) z = add2(z, rs);
-            if (BORDER != BORDER_AS_IT_IS && act == ACT_RELU) {
-                const float2 of = mul2(xs, a[j]);
-                const bool first = fabsf(z.x) < NEAR_BORDER * (fabsf(of.x) + fabsf(rs.x)), second = VN > 1 && fabsf(z.y) < NEAR_BORDER * (fabsf(of.y) + fabsf(rs.y));
-                near |= first | second;
-                if (BORDER == BORDER_SETTLED && first) z.x = exact_argument(p, s, channel_of(p, c0 + 2 * (j0 + j)), xs.x, rs.x);
-                if (BORDER == BORDER_SETTLED && second) z.y = exact_argument(p, s, channel_of(p, c0 + 2 * (j0 + j) + 1), xs.y, rs.y);
-            }
+            if (SETTLED && act == ACT_RELU)
+                settle<VN>(p, s, c0 + 2 * (j0 + j), xs, b[j], rs, z);
             const float2 v = act2_backward(act, z, pair_of(g.v[u], j0 + j));
             out[j] = (DROP < 0 ? p.drop.on : DROP) ? drop2<VN>(p, words[u], j0 + j, v) : v;
         }
-        return near;
     }
 };
 template <typename T, int VN>
@@ -691,7 +740,7 @@ __device__ __forceinline__ void bwd_sums_piece(const NormAct &p, const Columns &
                     if (r + u * l.lanes < n)
                     {
                         float2 xc[PAIRS], gz[PAIRS];
-                        in.template gz<PAIRS, BORDER_SETTLED>(p, s, lump * VN, u, h * PAIRS, mu, fa, fb, xc, gz);
+                        in.template gz<PAIRS, true>(p, s, lump * VN, u, h * PAIRS, mu, fa, fb, xc, gz);
 #pragma unroll
                         for (int i = 0; i < PAIRS; ++i) a[h * PAIRS + i] = add2(a[h * PAIRS + i], gz[i]), b[h * PAIRS + i] = fma2(gz[i], xc[i], b[h * PAIRS + i]);
                     }
@@ -727,7 +776,8 @@ __device__ __forceinline__ bool bwd_apply_piece(const NormAct &p, const Columns 
 #pragma unroll
                 for (int u = 0; u < U; ++u) {
                     float2 xc[PAIRS], gz[PAIRS];
-                    in.template gz<PAIRS, BORDER_AS_IT_IS>(p, s, lump * VN, u, h * PAIRS, mu, fa, fb, xc, gz);
+                    if (r + u * l.lanes < n) in.template gz<PAIRS, true>(p, s, lump * VN, u, h * PAIRS, mu, fa, fb, xc, gz);
+                    else continue;
 #pragma unroll
                     for (int i = 0; i < PAIRS; ++i) {
                         const int j = h * PAIRS + i;
@@ -968,12 +1018,22 @@ struct __align__(16) Tile {
     int first, whole;            // and a lump is the sample's, whole, if its place less `first` is below `whole`
 };
 struct Piece { int kind, s, chunk, rows; };
+// A warp of workers that has lumps with a ReLU's argument next to its border in a tile asks the clerk to settle them, and waits: (the tile's
+// place and its round's parity) * 4 + one of these.
+enum { ASK_NOTHING = 0, ASK_SUMS = 1, ASK_APPLY = 2, ASK_ANSWERED = 3 };
+// What passes between them, in the room of merge_groups (no block merges while one of its warps is at a tile).
+struct Asked {
+    uint32_t rounds[NA_THREADS];   // bit i: the i-th of the thread's rows in the tile
+    float2 sums[8][32];            // the answer: what those lumps add to a channel's sums
+};
+static_assert(sizeof(Asked) <= NA_THREADS * sizeof(double2), "room");
 
 struct Ring {
     uint64_t full[RING_STAGES], empty[RING_STAGES], folded[FOLD_SLOTS], taken[FOLD_SLOTS];
     Tile tiles[RING_STAGES];
     Piece pieces[FOLD_SLOTS];
     int told, abort;
+    volatile int asked[NA_THREADS / 32];   // of the clerk, by the workers' warps (enum above)
 };
 // Whether whole rows of columns make a warp (64 channels: 8 columns, 4 rows): its lanes are then folded before the clerk has them.
 __host__ __device__ __forceinline__ bool warps_fold(const Columns &l) { return l.cols < 32 && 32 % l.cols == 0; }
@@ -1118,8 +1178,107 @@ __device__ __forceinline__ void ring_producer(const NormAct &p, Ring &ring, cons
     }
 }
 
+// Of a pair at `at`, what is within first <= at < end.
+__device__ __forceinline__ float2 within(float2 v, int at, int first, int end) {
+    return make_float2(at >= first && at < end ? v.x : 0.f, at + 1 >= first && at + 1 < end ? v.y : 0.f);
+}
+
+// The clerk's answer to warp `w`: lane for lane what its threads would do, with the arguments' signs settled.  Lumps were left out of the sums; of
+// the results they are written once more.  Few elements come here (with a residual some ten of 70 million), but all may: values of 16
+// bits come again, and a channel's border may lie at one of them.  (The workers do not do it themselves: whatever they would hold
+// for it costs all other elements registers.  1.1 million points of 64 channels, bf16, residual, backward: 256 us where they do, 280 by a
+// call.)
+template <typename T, int DROP, bool PHASES>
+__device__ __forceinline__ void settle_tile(const NormAct &p, Ring &ring, const RingMemory &m, int w) {
+    constexpr int VN = 8;
+    const int lane = threadIdx.x & 31, request = ring.asked[w], kind = request & 3, parity = request >> 2 & 1, place = request >> 3;
+    Asked &asked = *reinterpret_cast<Asked *>(m.scratch);
+    __threadfence_block();
+    tc::mbar_wait(tc::smem_u32(&ring.full[place]), parity, NA_STATUS, p.status);   // (is there: the tile's bytes are this warp's to read, too)
+    __syncwarp();
+    const Tile &t = ring.tiles[place];
+    const Columns l(p.V, VN, 32 * w + lane);
+    const Philox<DROP != 1> rng(p.drop);
+    const int c0 = l.col * VN, tensor = p.tile_rows * p.V, s = t.s;
+    const T *x = reinterpret_cast<const T *>(m.stages + (size_t)place * p.stage_bytes) + c0;
+    Constants<VN, true> k;
+    k.at = m.constants + (kind == ASK_SUMS ? 5 * p.V : 0);
+    float2 a[4], b[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) a[j] = b[j] = both(0.f);
+    uint32_t rounds = asked.rounds[32 * w + lane];
+    for (int at = l.lane * p.V; rounds; rounds >>= 1, at += l.lanes * p.V) {
+        if (!(rounds & 1)) continue;
+        const int64_t to = t.from + at + c0;
+        const int first = PHASES ? t.first - at - c0 : 0, end = PHASES ? t.end - at - c0 : VN;
+        BackwardRows<T, VN, ACT_RELU, DROP, 1> in;
+        in.x.v[0].load(x + at);
+        in.g.v[0].load(x + tensor + at);
+        if (p.residual) in.res.v[0].load(x + 2 * tensor + at);
+        if (DROP) rng.template words<VN>((uint64_t)to, in.words[0]);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            float2 mu[2], fa[2], fb[2], m1[2], m2[2];
+            k.read(l, K_MU, h, mu), k.read(l, K_A, h, fa), k.read(l, K_B, h, fb);
+            if (kind == ASK_APPLY) k.read(l, K_M1, h, m1), k.read(l, K_M2, h, m2);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int j = 2 * h + i;
+                const float2 xs = pair_of(in.x.v[0], j), rs = p.residual ? pair_of(in.res.v[0], j) : both(0.f), xc = add2(xs, mu[i]);
+                float2 z = fma2(xc, fa[i], fb[i]);
+                if (p.residual) z = add2(z, rs);
+                settle<VN>(p, s, c0 + 2 * j, xs, fb[i], rs, z);
+                z = act2_backward(ACT_RELU, z, pair_of(in.g.v[0], j));
+                if (DROP) z = drop2<VN>(p, in.words[0], j, z);
+                if (kind == ASK_APPLY) {
+                    set_pair(in.g.v[0], j, z), set_pair(in.x.v[0], j, fma2(z, fa[i], fma2(xc, m2[i], m1[i])));
+                } else {
+                    z = within(z, 2 * j, first, end);
+                    a[j] = add2(a[j], z), b[j] = fma2(z, within(xc, 2 * j, first, end), b[j]);
+                }
+            }
+        }
+        if (kind == ASK_APPLY) {
+            if (p.dresidual) in.g.v[0].store_part(static_cast<T *>(p.dresidual) + to, first, end);
+            in.x.v[0].store_part(static_cast<T *>(p.dx) + to, first, end);
+        }
+    }
+    if (kind == ASK_SUMS) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) asked.sums[2 * j][lane] = a[j], asked.sums[2 * j + 1][lane] = b[j];
+    }
+    __threadfence_block();
+    __syncwarp();
+    if (lane == 0) ring.asked[w] = kind == ASK_SUMS ? ASK_ANSWERED : ASK_NOTHING;
+    if (kind == ASK_SUMS) {   // the next answer takes the place of this one: until it has been read
+        const uint64_t t0 = tc::global_timer_ns();
+        while (ring.asked[w] == ASK_ANSWERED && !*const_cast<volatile int *>(&ring.abort) && tc::global_timer_ns() - t0 <= tc::WAIT_LIMIT_NS) __nanosleep(20);
+    }
+    __syncwarp();
+}
+
+// Until a piece's sums are there; meanwhile warps that ask are answered.  False: a wait has run out.
+template <typename T, int DROP, bool PHASES>
+__device__ __forceinline__ bool answer_until_folded(const NormAct &p, Ring &ring, const RingMemory &m, const Place &slot) {
+    const int lane = threadIdx.x & 31;
+    for (uint64_t t0 = tc::global_timer_ns();;) {
+        if (__all_sync(0xffffffffu, tc::mbar_try_wait_parked(tc::smem_u32(&ring.folded[slot.at]), slot.parity, 500u))) return true;
+        const int asked = lane < NA_THREADS / 32 ? ring.asked[lane] & 3 : ASK_NOTHING;
+        unsigned warps = __ballot_sync(0xffffffffu, asked == ASK_SUMS || asked == ASK_APPLY);
+        if (warps) {
+            for (; warps; warps &= warps - 1) settle_tile<T, DROP, PHASES>(p, ring, m, __ffs(warps) - 1);
+            t0 = tc::global_timer_ns();
+        }
+        const bool late = tc::global_timer_ns() - t0 > tc::WAIT_LIMIT_NS, over = *const_cast<volatile int *>(&ring.abort);
+        if (__any_sync(0xffffffffu, late || over)) {
+            if (lane == 0 && !over) ring.abort = 1, atomicOr(p.status, NA_STATUS);
+            return false;
+        }
+    }
+}
+
 // Folds the sums of pieces over the row lanes and takes them from there.
-template <bool BACKWARD, bool PHASES>
+template <typename T, int ACT, int DROP, bool BACKWARD, bool PHASES>
 __device__ __forceinline__ void ring_clerk(const NormAct &p, Ring &ring, const RingMemory &m) {
     const int lane = threadIdx.x & 31;
     const Columns l(p.V, 8, 0);
@@ -1132,7 +1291,11 @@ __device__ __forceinline__ void ring_clerk(const NormAct &p, Ring &ring, const R
     Place slot;
     for (;;) {
         slot.next(folds.slots);
-        if (!__all_sync(0xffffffffu, tc::mbar_wait_abortable(tc::smem_u32(&ring.folded[slot.at]), slot.parity, NA_STATUS, p.status, &ring.abort))) return;
+        if constexpr (BACKWARD && ACT == ACT_RELU) {
+            if (!answer_until_folded<T, DROP, PHASES>(p, ring, m, slot)) return;
+        } else {
+            if (!__all_sync(0xffffffffu, tc::mbar_wait_abortable(tc::smem_u32(&ring.folded[slot.at]), slot.parity, NA_STATUS, p.status, &ring.abort))) return;
+        }
         const Piece piece = ring.pieces[slot.at];
         if (piece.kind == TILE_END) return;
         Two *fold = reinterpret_cast<Two *>(m.fold) + slot.at * 8 * folds.stride;
@@ -1172,55 +1335,11 @@ __device__ __forceinline__ void ring_clerk(const NormAct &p, Ring &ring, const R
     }
 }
 
-// Of a pair at `at`, what is within first <= at < end.
-__device__ __forceinline__ float2 within(float2 v, int at, int first, int end) {
-    return make_float2(at >= first && at < end ? v.x : 0.f, at + 1 >= first && at + 1 < end ? v.y : 0.f);
-}
-
-// Sums of a thread, less what the lump at `from` gave them and more what it gives with its arguments' signs settled.
-struct TwoSums { float2 a[4], b[4]; };
-template <typename T, int DROP, bool PHASES>
-__device__ __noinline__ void settle_sums(const NormAct &p, int64_t from, int64_t s, int chunk, int c0, TwoSums *sums) {
-    BackwardRows<T, 8, ACT_RELU, DROP, 1> in;
-    int first = 0, end = 8;
-    if constexpr (PHASES) {
-        const int64_t row0 = max((int64_t)chunk * p.rows, p.offsets[s]), row1 = min((int64_t)(chunk + 1) * p.rows, p.offsets[s + 1]);
-        first = (int)max(row0 * p.C - from, (int64_t)0), end = (int)min(row1 * p.C - from, (int64_t)8);
-        for (int i = 0; i < 8; ++i) {
-            const bool ours = i >= first && i < end;
-            in.x.v[0].set(i, ours ? to_f32<T>(static_cast<const T *>(p.x)[from + i]) : 0.f), in.g.v[0].set(i, ours ? to_f32<T>(static_cast<const T *>(p.g)[from + i]) : 0.f);
-            if (p.residual) in.res.v[0].set(i, ours ? to_f32<T>(static_cast<const T *>(p.residual)[from + i]) : 0.f);
-        }
-    } else {
-        in.x.v[0].load(static_cast<const T *>(p.x) + from), in.g.v[0].load(static_cast<const T *>(p.g) + from);
-        if (p.residual) in.res.v[0].load(static_cast<const T *>(p.residual) + from);
-    }
-    if (DROP) Philox<DROP != 1>(p.drop).template words<8>((uint64_t)from, in.words[0]);
-    float2 mu[4], a[4], b[4], xc[4], before[4], after[4];
-    for (int j = 0; j < 4; ++j) {
-        float v[6];
-        for (int i = 0; i < 2; ++i) {   // (as Constants::load makes them)
-            const int c = PHASES ? channel_of(p, c0 + 2 * j + i) : c0 + 2 * j + i;
-            const int64_t g = s * p.G + group_of(p, c);
-            const Mapping map(__ldg(p.mean + g), __ldg(p.rstd + g), p.weight ? __ldg(p.weight + c) : 1.f, p.weight ? __ldg(p.bias + c) : 0.f);
-            v[i] = -map.mu, v[2 + i] = map.a, v[4 + i] = map.b;
-        }
-        mu[j] = make_float2(v[0], v[1]), a[j] = make_float2(v[2], v[3]), b[j] = make_float2(v[4], v[5]);
-    }
-    in.template gz<4, BORDER_AS_IT_IS>(p, s, c0, 0, 0, mu, a, b, xc, before);
-    in.template gz<4, BORDER_SETTLED>(p, s, c0, 0, 0, mu, a, b, xc, after);
-    for (int j = 0; j < 4; ++j) {
-        float2 more = add2(after[j], neg2(before[j]));
-        if (PHASES) more = within(more, 2 * j, first, end);
-        sums->a[j] = add2(sums->a[j], more), sums->b[j] = fma2(more, xc[j], sums->b[j]);
-    }
-}
-
 // The workers' warps wait for tiles each by itself, and meet where the sample changes.  One whose wait has run out comes to the next
 // meeting with that, whichever it is, and then all of them leave: a meeting is the first barrier that a warp comes to after any tile.
 template <typename T, int ACT, int DROP, bool BACKWARD, bool PHASES>
 __device__ __forceinline__ void ring_worker(const NormAct &p, Ring &ring, const RingMemory &m) {
-    constexpr int VN = 8, P = 4, UNROLL = BACKWARD && DROP ? 1 : 2;   // (more spills registers)
+    constexpr int VN = 8, P = 4, UNROLL = BACKWARD && (DROP || ACT == ACT_RELU) ? 1 : 2;   // (more spills registers)
     const Columns l(p.V, VN, threadIdx.x);
     const Folds<BACKWARD> folds(l);
     using Two = typename Folds<BACKWARD>::Two;
@@ -1263,6 +1382,23 @@ __device__ __forceinline__ void ring_worker(const NormAct &p, Ring &ring, const 
         if (threadIdx.x == 0) ring.pieces[slot.at] = piece;
         __syncwarp();
         if ((threadIdx.x & 31) == 0) tc::mbar_arrive(tc::smem_u32(&ring.folded[slot.at]));
+    };
+    // Has the clerk settle the tile's lumps of these rounds; false: it did not come.
+    const auto ask = [&](int kind, uint32_t rounds) -> bool {
+        const int w = threadIdx.x >> 5;
+        reinterpret_cast<Asked *>(m.scratch)->rounds[threadIdx.x] = rounds;
+        __threadfence_block();   // (what has been written of the results is overwritten)
+        __syncwarp();
+        if ((threadIdx.x & 31) == 0) ring.asked[w] = (place.at * 2 + place.parity) * 4 + kind;
+        __syncwarp();
+        const int answered = kind == ASK_SUMS ? ASK_ANSWERED : ASK_NOTHING;
+        const uint64_t t0 = tc::global_timer_ns();
+        bool there = false;
+        while (!(there = ring.asked[w] == answered) && tc::global_timer_ns() - t0 <= tc::WAIT_LIMIT_NS) __nanosleep(50);
+        there = __all_sync(0xffffffffu, there);
+        if (!there && (threadIdx.x & 31) == 0) atomicOr(p.status, NA_STATUS);
+        __threadfence_block();
+        return there;
     };
     // A piece's sums, `part(i)` those of the lump's channels, into its slot: over the warp's row lanes first, where that is whole.
     const auto fold_and_send = [&](const Piece &piece, auto part) {
@@ -1329,7 +1465,6 @@ __device__ __forceinline__ void ring_worker(const NormAct &p, Ring &ring, const 
         } else if (t.kind == TILE_SUMS) {
             float2 a[P], b[P], mu[P], fa[P], fb[P];
             const int s = t.s, chunk = t.chunk;
-            int64_t unsettled = -1;   // a lump with a ReLU's argument next to its border (of two in a thread's part of a piece, the last)
             if (k_sums.s != s) {
                 if (!sync_workers_and(true)) break;
                 k_sums.template load<PHASES>(p, l, s, 0, false);
@@ -1338,19 +1473,22 @@ __device__ __forceinline__ void ring_worker(const NormAct &p, Ring &ring, const 
 #pragma unroll
             for (int j = 0; j < P; ++j) a[j] = b[j] = both(0.f);
             k_sums.read_all(l, K_MU, mu), k_sums.read_all(l, K_A, fa), k_sums.read_all(l, K_B, fb);
+            const float b_most = ACT == ACT_RELU ? largest(fb) : 0.f;
             int rows = 0;
             for (bool more = true; more;) {
                 const T *x = rows_at();
+                uint32_t unsettled = 0, round = 1;
                 if (mine)
 #pragma unroll UNROLL
-                    for (int r = l.lane, at = l.lane * p.V; r < t.n; r += l.lanes, at += step) {
+                    for (int r = l.lane, at = l.lane * p.V; r < t.n; r += l.lanes, at += step, round <<= 1) {
                         BackwardRows<T, VN, ACT, DROP, 1> in;
                         in.x.v[0].load(x + at);
                         in.g.v[0].load(x + tensor + at);
                         if (p.residual) in.res.v[0].load(x + 2 * tensor + at);
                         if (DROP) rng.template words<VN>((uint64_t)(t.from + at + c0), in.words[0]);
                         float2 xc[P], gz[P];
-                        if (in.template gz<P, ACT == ACT_RELU ? BORDER_TOLD : BORDER_AS_IT_IS>(p, s, c0, 0, 0, mu, fa, fb, xc, gz)) unsettled = t.from + at + c0;
+                        if constexpr (ACT == ACT_RELU) unsettled |= in.template gz_told<true>(p, b_most, mu, fa, fb, xc, gz) ? round : 0;
+                        else in.template gz<P, false>(p, s, c0, 0, 0, mu, fa, fb, xc, gz);
                         if (PHASES && cut(at + c0)) {
                             const int2 e = ends();
 #pragma unroll
@@ -1359,24 +1497,24 @@ __device__ __forceinline__ void ring_worker(const NormAct &p, Ring &ring, const 
 #pragma unroll
                         for (int j = 0; j < P; ++j) a[j] = add2(a[j], gz[j]), b[j] = fma2(gz[j], xc[j], b[j]);
                     }
+                bool lost = false;
+                if constexpr (ACT == ACT_RELU && BACKWARD)
+                    if (__any_sync(0xffffffffu, unsettled != 0)) {
+                        lost = !ask(ASK_SUMS, unsettled);
+                        const Asked &asked = *reinterpret_cast<const Asked *>(m.scratch);
+#pragma unroll
+                        for (int j = 0; j < P; ++j) a[j] = add2(a[j], asked.sums[2 * j][threadIdx.x & 31]), b[j] = add2(b[j], asked.sums[2 * j + 1][threadIdx.x & 31]);
+                        __syncwarp();
+                        if ((threadIdx.x & 31) == 0) ring.asked[threadIdx.x >> 5] = ASK_NOTHING;
+                    }
                 rows = t.last;
                 more = !rows;
                 release();
                 next_tile();
+                if (lost) t.kind = TILE_NONE;
                 if (t.kind == TILE_NONE) more = false;
             }
             if (!free) t.kind = TILE_NONE;
-            if constexpr (ACT == ACT_RELU) {
-                if (unsettled >= 0) {
-                    TwoSums sums;
-#pragma unroll
-                    for (int j = 0; j < P; ++j) sums.a[j] = a[j], sums.b[j] = b[j];
-                    settle_sums<T, DROP, PHASES>(p, unsettled, s, chunk, c0, &sums);
-#pragma unroll
-                    for (int j = 0; j < P; ++j) a[j] = sums.a[j], b[j] = sums.b[j];
-                }
-                __syncwarp();
-            }
             if constexpr (BACKWARD)
                 if (t.kind != TILE_NONE)
                     fold_and_send(Piece{TILE_SUMS, s, chunk, rows}, [&](int i) { return i % 2 ? make_float2(a[i / 2].y, b[i / 2].y) : make_float2(a[i / 2].x, b[i / 2].x); });
@@ -1389,12 +1527,14 @@ __device__ __forceinline__ void ring_worker(const NormAct &p, Ring &ring, const 
             float2 mu[P], fa[P], fb[P], m1[P], m2[P];
             k_apply.read_all(l, K_MU, mu), k_apply.read_all(l, K_A, fa), k_apply.read_all(l, K_B, fb);
             if constexpr (BACKWARD) k_apply.read_all(l, K_M1, m1), k_apply.read_all(l, K_M2, m2);
+            const float b_most = ACT == ACT_RELU ? largest(fb) : 0.f;
             do {
                 const T *x = rows_at();
                 if (!BACKWARD && t.last) k_apply.put_stats(p, l);
+                uint32_t unsettled = 0, round = 1;
                 if (mine)
 #pragma unroll UNROLL
-                    for (int r = l.lane, at = l.lane * p.V; r < t.n; r += l.lanes, at += step) {
+                    for (int r = l.lane, at = l.lane * p.V; r < t.n; r += l.lanes, at += step, round <<= 1) {
                         const int64_t to = t.from + at + c0;
                         BackwardRows<T, VN, ACT, DROP, 1> in;
                         in.x.v[0].load(x + at);
@@ -1402,7 +1542,8 @@ __device__ __forceinline__ void ring_worker(const NormAct &p, Ring &ring, const 
                         if (p.residual) in.res.v[0].load(x + (BACKWARD ? 2 : 1) * tensor + at);
                         if (DROP) rng.template words<VN>((uint64_t)to, in.words[0]);
                         float2 xc[P], gz[P];
-                        if constexpr (BACKWARD) in.template gz<P, BORDER_AS_IT_IS>(p, s, c0, 0, 0, mu, fa, fb, xc, gz);
+                        if constexpr (BACKWARD && ACT == ACT_RELU) unsettled |= in.template gz_told<false>(p, b_most, mu, fa, fb, xc, gz) ? round : 0;
+                        else if constexpr (BACKWARD) in.template gz<P, false>(p, s, c0, 0, 0, mu, fa, fb, xc, gz);
 #pragma unroll
                         for (int j = 0; j < P; ++j) {
                             if constexpr (BACKWARD) {
@@ -1425,8 +1566,12 @@ __device__ __forceinline__ void ring_worker(const NormAct &p, Ring &ring, const 
                             in.x.v[0].store_streaming(static_cast<T *>(BACKWARD ? p.dx : p.y) + to);
                         }
                     }
+                bool lost = false;
+                if constexpr (ACT == ACT_RELU && BACKWARD)
+                    if (__any_sync(0xffffffffu, unsettled != 0)) lost = !ask(ASK_APPLY, unsettled);
                 release();
                 next_tile();
+                if (lost) t.kind = TILE_NONE;
             } while (t.kind == TILE_APPLY && t.s == s);
         } else {
             if (!sync_workers_and(t.kind != TILE_NONE)) break;
@@ -1454,6 +1599,7 @@ __global__ void __launch_bounds__(RING_THREADS, RING_BLOCKS) na_ring_kernel(cons
         for (int q = 0; q < p.stages; ++q) tc::mbar_init(tc::smem_u32(&ring.full[q]), 1), tc::mbar_init(tc::smem_u32(&ring.empty[q]), NA_THREADS / 32);
         for (int q = 0; q < FOLD_SLOTS; ++q) tc::mbar_init(tc::smem_u32(&ring.folded[q]), NA_THREADS / 32), tc::mbar_init(tc::smem_u32(&ring.taken[q]), 1);
         ring.abort = 0;
+        for (int w = 0; w < NA_THREADS / 32; ++w) ring.asked[w] = ASK_NOTHING;
         tc::fence_mbar_init();
     }
     start_after_previous();
@@ -1461,7 +1607,7 @@ __global__ void __launch_bounds__(RING_THREADS, RING_BLOCKS) na_ring_kernel(cons
     const RingMemory m(p, shared);
     if (threadIdx.x < NA_THREADS) ring_worker<T, ACT, DROP, BACKWARD, PHASES>(p, ring, m);
     else if (threadIdx.x < NA_THREADS + 32) ring_producer<T, BACKWARD, PHASES>(p, ring, m);
-    else ring_clerk<BACKWARD, PHASES>(p, ring, m);
+    else ring_clerk<T, ACT, DROP, BACKWARD, PHASES>(p, ring, m);
 }
 
 template <typename T, int ACT, int DROP, bool BACKWARD, bool PHASES>

@@ -55,3 +55,65 @@ def test_far_from_zero(far, C, G, residual):
     assert bool(((dx.double() - want).abs() <= 16 * e * size).all())
     dw_want, dw_size = (go.double() * xh).sum(0), (go.double() * xh).abs().sum(0)
     assert bool(((dw.double() - dw_want).abs() <= 16 * e * dw_size).all())
+
+
+def _at_the_border(lengths, C, G, dtype, residual, seed):
+    """Values of a few steps of the type, as layers of 16 bits have them, and a bias that puts one of them, a few rows in a hundred,
+    on the border of the ReLU, so near that 32 bits do not tell on which side: z is what the bias's rounding leaves."""
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    N = sum(lengths)
+    values = torch.tensor([0.0, 1.0, -2.0, 0.5, 3.0, -0.75, 100.0], device=DEV)
+    x = values[torch.randint(0, 7, (N, C), generator=g, device=DEV)].to(dtype)
+    res = values[torch.randint(0, 3, (N, C), generator=g, device=DEV)].to(dtype) if residual else None
+    w = 1 + 0.2 * torch.randn(C, generator=g, device=DEV)
+    zero = torch.zeros(C, device=DEV)
+    _, _, xh, _ = _definition(x, lengths, G, w, zero, None)
+    at = torch.arange(C, device=DEV) % 7       # the value that is on the border, in the batch's first sample
+    first = x[:lengths[0]].float()
+    row = (first == values[at].to(dtype).float()).int().argmax(0)
+    b = -(xh[row, torch.arange(C, device=DEV)] * w.double())
+    if residual:
+        b = b - values[1].double()             # with a residual of one
+    return x, res, w, b.float()
+
+
+@pytest.mark.parametrize("C,G,lengths", [(64, 8, [3001, 700]), (64, 64, [20000]), (50, 5, [3001, 3, 700]), (33, 1, [2500, 1]), (1032, 4, [900, 80]), (256, 256, [5000, 9])])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("residual,p", [(False, 0.0), (True, 0.0), (True, 0.3), (False, 0.3)])
+def test_signs_at_the_border(C, G, lengths, dtype, residual, p):
+    """Every element of the gradients of x and of the residual, and of the sums, is on the side that float64 gives it; y is the ReLU of an
+    argument that is off by some 2^-22 of its terms."""
+    import numpy as np
+
+    from oracle import norm_act as oracle
+    from pointelligence_b200.layers.norm import fused_group_norm_act
+
+    x, res, w, b = _at_the_border(lengths, C, G, dtype, residual, C)
+    N = sum(lengths)
+    go = (1 + torch.rand(N, C, device=DEV)).to(dtype)      # (no gradient is zero)
+    leaves = [t.requires_grad_() for t in (x, w, b)] + ([res.requires_grad_()] if residual else [])
+    y = fused_group_norm_act(x, torch.tensor(lengths, device=DEV), G, w, b, residual=res, activation="relu", dropout=p, rng=(5, 8) if p else None)
+    grads = torch.autograd.grad(y, leaves, go)
+    _, rstd, xh, z = _definition(x.detach(), lengths, G, w.detach(), b.detach(), None if res is None else res.detach())
+    near = z.abs() < 2.0 ** -22
+    assert 0.002 < float(near.double().mean())
+    # (a constant row or group has z = 0 but for the order of float64's sums)
+    told = z.abs() > 2.0 ** -45
+    keep = torch.from_numpy(oracle.keep_factor(np.arange(N * C), p, (5, 8))).view(N, C).to(DEV) if p else torch.ones(N, C, dtype=torch.double, device=DEV)
+    open_ = (z > 0) & (keep > 0)
+    y_want, terms = z.clamp_min(0) * keep, (xh * w.detach().double()).abs() + b.detach().double().abs() + (0 if res is None else res.detach().double().abs())
+    assert bool(((y.detach().double() - y_want).abs() <= U[dtype] * y_want + 2.0 ** -22 * terms * keep + 2.0 ** -24 * (dtype == torch.float16)).all())
+    if residual:
+        assert torch.equal((grads[3] != 0)[told], open_[told])
+    gz = go.double() * keep * open_
+    unsure = (go.double() * keep * ~told).sum(0)
+    size = gz.sum(0)
+    # sums of 32 bits in short chains: 16 roundings of 2^-24 of their terms, as many for each part of xh
+    assert bool(((grads[2].double() - size).abs() <= 2.0 ** -20 * size + unsure).all())
+    assert bool(((grads[1].double() - (gz * xh).sum(0)).abs() <= 2.0 ** -20 * (gz * xh.abs()).sum(0) + unsure * xh.abs().max()).all())
+    by_group = lambda t: torch.cat([q.view(len(q), G, -1).mean((0, 2), keepdim=True).expand(len(q), G, C // G).reshape(len(q), C) for q in torch.split(t, lengths)])
+    gh = gz * w.detach().double()
+    dx = rstd * (gh - by_group(gh) - xh * by_group(gh * xh))
+    loose = rstd * (by_group(go.double() * keep * ~told * w.detach().double().abs()) * (1 + xh.abs() * xh.abs().max()))
+    bound = U[dtype] * dx.abs() + 2.0 ** -19 * rstd * (gh.abs() + by_group(gh.abs()) + xh.abs() * by_group((gh * xh).abs())) + loose + 2.0 ** -24
+    assert bool(((grads[0].double() - dx).abs() <= bound)[told].all())
