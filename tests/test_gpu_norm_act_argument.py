@@ -117,3 +117,44 @@ def test_signs_at_the_border(C, G, lengths, dtype, residual, p):
     loose = rstd * (by_group(go.double() * keep * ~told * w.detach().double().abs()) * (1 + xh.abs() * xh.abs().max()))
     bound = U[dtype] * dx.abs() + 2.0 ** -19 * rstd * (gh.abs() + by_group(gh.abs()) + xh.abs() * by_group((gh * xh).abs())) + loose + 2.0 ** -24
     assert bool(((grads[0].double() - dx).abs() <= bound)[told].all())
+
+
+def _values(kind, z):
+    """act(z) and its slope, in float64 on the host, from functions that are right in the tails."""
+    import numpy as np
+    from scipy import special
+
+    if kind == "silu":
+        s = special.expit(z)
+        return z * s, s * (1 + z * special.expit(-z)), s * (1 + np.abs(z) * special.expit(-z))
+    density = np.exp(-z * z / 2) / np.sqrt(2 * np.pi)
+    cdf = special.ndtr(z)
+    return z * cdf, cdf + z * density, cdf + np.abs(z) * density
+
+
+def _activated(kind, z, dtype):
+    """y and the residual's gradient for arguments z: the offsets of channels whose weight is zero."""
+    from pointelligence_b200.layers.norm import fused_group_norm_act
+
+    C = len(z)
+    x = torch.randn(4, C, device=DEV).to(dtype)
+    res = torch.zeros(4, C, device=DEV, dtype=dtype, requires_grad=True)
+    y = fused_group_norm_act(x, torch.tensor([4], device=DEV), 8, torch.zeros(C, device=DEV), torch.tensor(z, device=DEV, dtype=torch.float32), residual=res, activation=kind)
+    g, = torch.autograd.grad(y, res, torch.ones_like(y))
+    return [t.detach().double().cpu().numpy() for t in (y, g)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("C", [1024, 2048])
+def test_gelu_in_its_tails(dtype, C):
+    """Relative to the value: 2^-20 of the approximation with the reciprocal and the exponential; the exponent z^2 / 2 is three roundings, 2^-23 z^2
+    of the result.  Below -12 results leave fp32's normal numbers."""
+    import numpy as np
+
+    z = np.linspace(-12, 12, C).astype(np.float32).astype(float)
+    y, g = _activated("gelu", z, dtype)
+    want, slope, terms = _values("gelu", z)
+    tiny = 2.0 ** -25 if dtype == torch.float16 else 0.0
+    e = 2.0 ** -20 + 2.0 ** -23 * z * z
+    assert (np.abs(y - want) <= (U[dtype] + e) * np.abs(want) + tiny).all()
+    assert (np.abs(g - slope) <= U[dtype] * np.abs(slope) + e * terms + tiny).all()
