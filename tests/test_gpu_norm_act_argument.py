@@ -158,3 +158,47 @@ def test_gelu_in_its_tails(dtype, C):
     e = 2.0 ** -20 + 2.0 ** -23 * z * z
     assert (np.abs(y - want) <= (U[dtype] + e) * np.abs(want) + tiny).all()
     assert (np.abs(g - slope) <= U[dtype] * np.abs(slope) + e * terms + tiny).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("C", [1024, 2048])
+def test_silu_in_its_tails(dtype, C):
+    """Relative to the value: 2^-20 of the reciprocal and the exponential with its products; the exponent is two roundings, 2^-23 |z|
+    of the result.  Below -86 results leave fp32's normal numbers."""
+    import numpy as np
+
+    z = np.linspace(-86, 86, C).astype(np.float32).astype(float)
+    y, g = _activated("silu", z, dtype)
+    want, slope, terms = _values("silu", z)
+    tiny = 2.0 ** -25 if dtype == torch.float16 else 0.0
+    e = 2.0 ** -20 + 2.0 ** -23 * np.abs(z)
+    assert (np.abs(y - want) <= (U[dtype] + e) * np.abs(want) + tiny).all()
+    assert (np.abs(g - slope) <= U[dtype] * np.abs(slope) + e * terms + tiny).all()
+    y, g = _activated("silu", np.array([-1e3, -100.0, -0.0, 0.0, 100.0, 1e3, 3e4, -3e4] * 2), dtype)
+    assert (y == np.array([0, 0, 0, 0, 100, 1000, float(torch.tensor(3e4).to(dtype)), 0] * 2)).all()
+    assert (g == np.array([0, 0, 0.5, 0.5, 1, 1, 1, 0] * 2)).all()
+
+
+@pytest.mark.parametrize("kind", ["relu", "silu"])
+@pytest.mark.parametrize("C", [24, 25, 1032])
+def test_not_a_number_stays_in_its_channel(kind, C):
+    """Instance norm: what is no number in one channel leaves its neighbours as they are, in both directions."""
+    from pointelligence_b200.layers.norm import fused_group_norm_act
+
+    x = torch.randn(500, C, device=DEV).bfloat16()
+    res, go = torch.randn_like(x), torch.randn_like(x)
+
+    def run(x, res):
+        x, res = x.clone().requires_grad_(), res.clone().requires_grad_()
+        y = fused_group_norm_act(x, torch.tensor([500], device=DEV), C, residual=res, activation=kind)
+        return (y.detach(),) + torch.autograd.grad(y, (x, res), go)
+
+    clean = run(x, res)
+    for value in (float("nan"), float("inf"), -float("inf")):
+        bad_x, bad_res = x.clone(), res.clone()
+        bad_x[7, 3::8] = value
+        bad_res[9, 6::8] = value
+        apart = torch.ones(C, dtype=torch.bool, device=DEV)
+        apart[3::8] = apart[6::8] = False
+        for a, b in zip(run(bad_x, bad_res), clean):
+            assert torch.equal(a[:, apart], b[:, apart])
