@@ -104,9 +104,6 @@ __device__ __forceinline__ float rcp(float v) {
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
     return r;
 }
-// 1 / v of both, with one reciprocal: the special function units give 16 results a clock and SM.  v in 1 .. 2^62.
-__device__ __forceinline__ float2 rcp2(float2 v) { return mul2(both(rcp(v.x * v.y)), make_float2(v.y, v.x)); }
-
 // 1 / (1 + exp(-z)): right to a part of its value for all z down to exp's range (zero from z = -87 on), as the reciprocal is of one number.
 // (One for two, by their product, wants exp(-z) bounded by 2^62, and takes as long: forward with dropout 134 us for 135, backward 230 for 221,
 // 1.1 million rows of 64 channels, bf16.)
@@ -128,9 +125,8 @@ __device__ __forceinline__ void normal2(float2 z, float2 &cdf, float2 &density) 
     constexpr float p[10] = {WIDE ? 0.125666827f : 0.129656136f,   WIDE ? 0.125665396f : 0.129672810f,  WIDE ? 0.113254927f : 0.115494095f,  WIDE ? 0.0873554945f : 0.0935735404f,
                              WIDE ? 0.0617356598f : 0.0258780140f, WIDE ? -0.0127292043f : 0.0855680779f, WIDE ? 0.0785122886f : -0.113720231f, WIDE ? -0.153162092f : 0.0338778943f,
                              WIDE ? 0.0932994485f : 0.f,           WIDE ? -0.0195987169f : 0.f};
-    const float2 a = make_float2(fminf(fabsf(z.x), 0x1p30f), fminf(fabsf(z.y), 0x1p30f));
-    const float2 t = rcp2(fma2(a, both(C), both(1.f)));
-    const float2 h = mul2(mul2(a, a), both(-0.5f * 1.4426950408889634f));
+    const float2 v = fma2(make_float2(fabsf(z.x), fabsf(z.y)), both(C), both(1.f)), t = make_float2(rcp(v.x), rcp(v.y));
+    const float2 h = mul2(mul2(z, z), both(-0.5f * 1.4426950408889634f));
     const float2 e = make_float2(ex2(h.x), ex2(h.y));   // exp(-z^2 / 2)
     float2 q = fma2(t, both(p[N - 1]), both(p[N - 2]));
 #pragma unroll

@@ -179,7 +179,7 @@ def test_silu_in_its_tails(dtype, C):
     assert (g == np.array([0, 0, 0.5, 0.5, 1, 1, 1, 0] * 2)).all()
 
 
-@pytest.mark.parametrize("kind", ["relu", "silu"])
+@pytest.mark.parametrize("kind", ["relu", "silu", "gelu"])
 @pytest.mark.parametrize("C", [24, 25, 1032])
 def test_not_a_number_stays_in_its_channel(kind, C):
     """Instance norm: what is no number in one channel leaves its neighbours as they are, in both directions."""
