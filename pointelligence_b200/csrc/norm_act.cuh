@@ -1049,7 +1049,7 @@ struct Folds {
     using Two = std::conditional_t<BACKWARD, float2, double2>;
     static constexpr int BYTES = 2 * 8 * (NA_THREADS + 2) * (int)sizeof(float2);
     int rows, stride, slots;   // rows of columns; from a channel of the lumps to the next, so that the clerk finds no bank conflicts
-    __device__ __forceinline__ explicit Folds(const Columns &l) {
+    __host__ __device__ __forceinline__ explicit Folds(const Columns &l) {
         rows = warps_fold(l) ? NA_THREADS / 32 : l.lanes;
         stride = BACKWARD ? NA_THREADS + 2 : rows * l.cols | 1;
         slots = BACKWARD || stride <= NA_THREADS / 2 + 1 ? FOLD_SLOTS : 1;
@@ -1072,7 +1072,8 @@ struct RingMemory {
     }
 };
 inline size_t ring_bytes(int V, int G, bool backward) {   // without the tiles
-    return (size_t)Folds<true>::BYTES + NA_THREADS * sizeof(double2) + (size_t)G * sizeof(Stats) + (size_t)(backward ? 8 : 3 + FOLD_SLOTS) * V * sizeof(float);
+    return (size_t)Folds<true>::BYTES + NA_THREADS * sizeof(double2) + (size_t)G * sizeof(Stats) +
+           (size_t)(backward ? 8 : 3 + Folds<false>(Columns(V, 8, 0)).slots + 1) * V * sizeof(float);
 }
 
 __device__ __forceinline__ void bulk_copy(uint32_t to, const void *from, uint32_t bytes, uint32_t bar, uint64_t policy) {
@@ -1294,7 +1295,7 @@ __device__ __forceinline__ void ring_clerk(const NormAct &p, Ring &ring, const R
     while (!few && 2 * parts * p.C <= 32) parts *= 2;
     const int share = lanes_of_group<WarpTeam>(p);
     Place slot;
-    for (;;) {
+    for (int pieces = 0;; ++pieces) {
         slot.next(folds.slots);
         if constexpr (BACKWARD && ACT == ACT_RELU) {
             if (!answer_until_folded<T, DROP, PHASES>(p, ring, m, slot)) return;
@@ -1304,7 +1305,7 @@ __device__ __forceinline__ void ring_clerk(const NormAct &p, Ring &ring, const R
         const Piece piece = ring.pieces[slot.at];
         if (piece.kind == TILE_END) return;
         Two *fold = reinterpret_cast<Two *>(m.fold) + slot.at * 8 * folds.stride;
-        const float *firsts = m.firsts + slot.at * p.V;
+        const float *firsts = m.firsts + pieces % (folds.slots + 1) * p.V;
         const int64_t number = piece.chunk + (int64_t)piece.s;
         const double inverse = 1.0 / piece.rows;
         for (int base = 0; base < p.C; base += 32 / parts) {   // (the same rounds for all lanes)
@@ -1378,7 +1379,7 @@ __device__ __forceinline__ void ring_worker(const NormAct &p, Ring &ring, const 
         if ((threadIdx.x & 31) == 0) tc::mbar_arrive(tc::smem_u32(&ring.empty[place.at]));
     };
     const auto rows_at = [&] { return reinterpret_cast<const T *>(m.stages + (size_t)place.at * p.stage_bytes) + c0; };
-    // A slot for sums; false: the clerk has not come for the ones before.
+    // A slot for sums, when they are ready; false: the clerk has not come for the ones before.
     const auto next_slot = [&]() -> bool {
         slot.next(folds.slots);
         return ++pieces <= folds.slots || __all_sync(0xffffffffu, tc::mbar_wait(tc::smem_u32(&ring.taken[slot.at]), slot.parity ^ 1, NA_STATUS, p.status));
@@ -1425,7 +1426,6 @@ __device__ __forceinline__ void ring_worker(const NormAct &p, Ring &ring, const 
     for (;;) {
         if (t.kind == TILE_SUMS && !BACKWARD) {
             const int s = t.s, chunk = t.chunk;
-            const bool free = next_slot();
             Lump<T, VN> k;
             if constexpr (PHASES) {
                 const T *first = rows_at() - c0 + ends().x;
@@ -1438,9 +1438,9 @@ __device__ __forceinline__ void ring_worker(const NormAct &p, Ring &ring, const 
             } else {
                 k.load(rows_at());
             }
-            if (l.lane == 0 && free) {   // (C of V are read)
+            if (l.lane == 0) {   // (C of V are read.  One more in turn than there are slots: the clerk may still be at all of those)
 #pragma unroll
-                for (int i = 0; i < VN; ++i) m.firsts[slot.at * p.V + c0 + i] = k.get(i);
+                for (int i = 0; i < VN; ++i) m.firsts[pieces % (folds.slots + 1) * p.V + c0 + i] = k.get(i);
             }
             Moments<VN> sums(k);
             int rows = 0;
@@ -1464,7 +1464,7 @@ __device__ __forceinline__ void ring_worker(const NormAct &p, Ring &ring, const 
                 next_tile();
                 if (t.kind == TILE_NONE) more = false;
             }
-            if (!free) t.kind = TILE_NONE;
+            if (!next_slot()) t.kind = TILE_NONE;
             if constexpr (!BACKWARD)
                 if (t.kind != TILE_NONE) fold_and_send(Piece{TILE_SUMS, s, chunk, rows}, [&](int i) { return make_double2(sums.a[i], sums.b[i]); });
         } else if (t.kind == TILE_SUMS) {
@@ -1474,7 +1474,6 @@ __device__ __forceinline__ void ring_worker(const NormAct &p, Ring &ring, const 
                 if (!sync_workers_and(true)) break;
                 k_sums.template load<PHASES>(p, l, s, 0, false);
             }
-            const bool free = next_slot();
 #pragma unroll
             for (int j = 0; j < P; ++j) a[j] = b[j] = both(0.f);
             k_sums.read_all(l, K_MU, mu), k_sums.read_all(l, K_A, fa), k_sums.read_all(l, K_B, fb);
@@ -1519,7 +1518,7 @@ __device__ __forceinline__ void ring_worker(const NormAct &p, Ring &ring, const 
                 if (lost) t.kind = TILE_NONE;
                 if (t.kind == TILE_NONE) more = false;
             }
-            if (!free) t.kind = TILE_NONE;
+            if (!next_slot()) t.kind = TILE_NONE;
             if constexpr (BACKWARD)
                 if (t.kind != TILE_NONE)
                     fold_and_send(Piece{TILE_SUMS, s, chunk, rows}, [&](int i) { return i % 2 ? make_float2(a[i / 2].y, b[i / 2].y) : make_float2(a[i / 2].x, b[i / 2].x); });
