@@ -795,7 +795,7 @@ struct Dropout : public torch::autograd::Function<Dropout> {
         const auto res_type = (at::ScalarType)ctx->saved_data["residual_type"].toInt();
         const auto given = [](const Tensor &t) { return t.defined() ? OptTensor(t) : std::nullopt; };
         if (!relu || at::GradMode::is_enabled()) {   // (the operator again: linear, and differentiable as often as asked for)
-            const Tensor g = relu ? grads[0] * (saved[0].detach() > 0) : grads[0];
+            const Tensor g = relu ? at::where(saved[0].detach() > 0, grads[0], 0) : grads[0];   // (no product: what the ReLU stops is zero, whatever it was)
             if (want_x) out[0] = dropout_with(g, given(saved[1]), std::nullopt, given(saved[2]), unit, false, p, sizes[2], sizes[3]);
             if (want_res) out[2] = g.to(res_type);
             return out;
