@@ -454,13 +454,16 @@ int pcx_ragged_group_norm_backward(const void *d_grad_y, const void *d_x,
 /* Group normalisation over a ragged batch with what follows it in a residual
  * block, in the same passes over the rows:
  *   y = drop(act((x - mean_{s,g}) * rstd_{s,g} * weight + bias (+ residual)))
- * G = 1 is the ragged layer norm, G = C the instance norm; C <= 65536.
+ * G = 1 is the ragged layer norm, G = C the instance norm; C <= 65536, and
+ * S * C is below 2^31.
  * `activation`: a pcx_activation.  `dropout` is the probability of the dropout
  * by element described at pcx_dropout (0: none).  d_weight / d_bias (fp32, C) may both
  * be null, and so may d_residual.  d_mean / d_rstd (fp64, S * G, index s * G + g)
  * are outputs kept for the backward pass, which makes the activation's argument and the
  * mask again: give it the tensors, the probability and the seed of the forward
- * call.  d_grad_weight / d_grad_bias (fp32, C) may both be null, and so may
+ * call.  The statistics are summed in fp64; in the backward pass a ReLU's
+ * argument that fp32 does not tell from zero has its sign from fp64.
+ * d_grad_weight / d_grad_bias (fp32, C) may both be null, and so may
  * d_grad_residual.  Results do not depend on scheduling: sums are merged in a
  * fixed order.  Lengths are taken within the rows there are; rows behind the
  * last sample are its own.  (layers/norm.py:86-130 of the reference composes the

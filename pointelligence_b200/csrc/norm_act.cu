@@ -135,8 +135,10 @@ size_t carve(void *ws, int64_t N, int64_t S, int C, int G, int dtype, NormAct *o
     return c.off;
 }
 
+bool too_many_samples(int64_t S, int C) { return S > 0 && C > 0 && S > INT32_MAX / C; }   // (counts of samples and windows are 32 bits, and no larger batch is tested)
+
 bool sizes_ok(int64_t N, int64_t S, int C, int G, int dtype, int activation) {
-    return N >= 0 && S > 0 && S <= INT32_MAX && C > 0 && C <= NA_MAX_C && G > 0 && C % G == 0 && S * (int64_t)C <= INT32_MAX &&
+    return N >= 0 && S > 0 && C > 0 && C <= NA_MAX_C && G > 0 && C % G == 0 && !too_many_samples(S, C) &&
            (dtype == PCX_F32 || dtype == PCX_F16 || dtype == PCX_BF16) && activation >= ACT_NONE && activation <= ACT_GELU &&
            (N == 0 || N <= INT64_MAX / 8 / C) && N / chunk_rows(std::max<int64_t>(N, 1), C, dtype) < INT32_MAX / 4;
 }
@@ -199,6 +201,7 @@ int pcx_ragged_group_norm_act(const void *d_x, const int64_t *d_lengths, const f
                               double *d_mean, double *d_rstd, int64_t N, int64_t S, int C, int G, double eps, int activation, double dropout, uint64_t seed,
                               uint64_t offset, const int64_t *d_rng, int dtype, void *d_ws, size_t ws_bytes, void *stream_) {
     cudaStream_t stream = (cudaStream_t)stream_;
+    if (too_many_samples(S, C)) PCX_FAIL(PCX_E_ARG, "pcx_ragged_group_norm_act: %lld samples of %d channels: S * C has to be below 2^31", (long long)S, C);
     if (!sizes_ok(N, S, C, G, dtype, activation))
         PCX_FAIL(PCX_E_ARG, "pcx_ragged_group_norm_act: bad sizes, activation or dtype (C <= %d must be a multiple of G)", NA_MAX_C);
     if (!d_lengths || !d_mean || !d_rstd || !d_ws || (N > 0 && (!d_x || !d_y)) || ((d_weight == nullptr) != (d_bias == nullptr)))
@@ -221,6 +224,7 @@ int pcx_ragged_group_norm_act_backward(const void *d_grad_y, const void *d_x, co
                                        float *d_grad_bias, void *d_grad_residual, int64_t N, int64_t S, int C, int G, int activation, double dropout,
                                        uint64_t seed, uint64_t offset, const int64_t *d_rng, int dtype, void *d_ws, size_t ws_bytes, void *stream_) {
     cudaStream_t stream = (cudaStream_t)stream_;
+    if (too_many_samples(S, C)) PCX_FAIL(PCX_E_ARG, "pcx_ragged_group_norm_act_backward: %lld samples of %d channels: S * C has to be below 2^31", (long long)S, C);
     if (!sizes_ok(N, S, C, G, dtype, activation))
         PCX_FAIL(PCX_E_ARG, "pcx_ragged_group_norm_act_backward: bad sizes, activation or dtype (C <= %d must be a multiple of G)", NA_MAX_C);
     if (!d_lengths || !d_mean || !d_rstd || !d_ws || (N > 0 && (!d_grad_y || !d_x || !d_grad_x)) || ((d_weight == nullptr) != (d_bias == nullptr)) ||
