@@ -563,31 +563,29 @@ __device__ __forceinline__ float exact_argument(const NormAct &p, int64_t s, int
     const double xh = ((double)x - __ldg(p.mean + g)) * __ldg(p.rstd + g);
     return (float)((p.weight ? xh * __ldg(p.weight + c) + __ldg(p.bias + c) : xh) + residual);
 }
+__device__ __noinline__ float exact_argument_call(const NormAct &p, int64_t s, int c, float x, float residual) { return exact_argument(p, s, c, x, residual); }
 // Settles a pair of arguments where they are next to the border.
+template <int VN>
+__device__ __forceinline__ void settle_by_call(const NormAct &p, int64_t s, int c, float2 x, float2 b, float2 residual, float2 &z) {
+    if (fabsf(z.x) < NEAR_BORDER * (fabsf(b.x) + fabsf(residual.x))) z.x = exact_argument_call(p, s, channel_of(p, c), x.x, residual.x);
+    if (VN > 1 && fabsf(z.y) < NEAR_BORDER * (fabsf(b.y) + fabsf(residual.y))) z.y = exact_argument_call(p, s, channel_of(p, c + 1), x.y, residual.y);
+}
 template <int VN>
 __device__ __forceinline__ void settle(const NormAct &p, int64_t s, int c, float2 x, float2 b, float2 residual, float2 &z) {
     if (fabsf(z.x) < NEAR_BORDER * (fabsf(b.x) + fabsf(residual.x))) z.x = exact_argument(p, s, channel_of(p, c), x.x, residual.x);
     if (VN > 1 && fabsf(z.y) < NEAR_BORDER * (fabsf(b.y) + fabsf(residual.y))) z.y = exact_argument(p, s, channel_of(p, c + 1), x.y, residual.y);
 }
-// Whether a ring's lump has such an argument, for the loops that all elements go through: its least one beside its largest offset (`b_most`: of
-// the thread's eight) and residual, and where that is near, one by one.  (Zeros of a channel without offset and residual are not near.)
-struct Least {
-    float z = INFINITY;
-    __device__ __forceinline__ void take(float2 v) { z = fminf(z, fminf(fabsf(v.x), fabsf(v.y))); }
-    // `residual(j)` of a pair; (a NaN in one channel: the others are looked at)
-    template <typename Residual>
-    __device__ __forceinline__ bool near(const float2 (&args)[4], const float2 *b, float b_most, float r_most, Residual residual) const {
-        if (z >= NEAR_BORDER * (b_most + r_most)) return false;
-        bool any = false;
+// Whether two pairs of arguments have such a one, for the loops that all elements go through: the least beside the largest offset (`b_most`: of
+// the thread's channels) and residual, and where that is near, one by one.  (Zeros of a channel without offset and residual are not near.
+// A NaN in one channel: the others are looked at.)
+__device__ __forceinline__ bool near_border(const float2 *z, const float2 *b, const float2 *residual, float b_most, float r_most) {
+    const float least = fminf(fminf(fabsf(z[0].x), fabsf(z[0].y)), fminf(fabsf(z[1].x), fabsf(z[1].y)));
+    if (least >= NEAR_BORDER * (b_most + r_most)) return false;
+    bool any = false;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float2 r = residual(j);
-            any |= fabsf(args[j].x) < NEAR_BORDER * (fabsf(b[j].x) + fabsf(r.x));
-            any |= fabsf(args[j].y) < NEAR_BORDER * (fabsf(b[j].y) + fabsf(r.y));
-        }
-        return any;
-    }
-};
+    for (int j = 0; j < 2; ++j) any |= fabsf(z[j].x) < NEAR_BORDER * (fabsf(b[j].x) + fabsf(residual[j].x)) || fabsf(z[j].y) < NEAR_BORDER * (fabsf(b[j].y) + fabsf(residual[j].y));
+    return any;
+}
 __device__ __forceinline__ float largest(const float2 (&v)[4]) {
     float m = 0.f;
 #pragma unroll
@@ -673,27 +671,28 @@ struct BackwardRows {
             for (int u = 0; u < U; ++u) rng.words<VN>((uint64_t)(from + (r + u * l.lanes) * p.C), words[u]);
         }
     }
-    // gz of a ring's lump, and whether it is next to a ReLU's border (then all zeros, if such are to be left out).
+    // x - mu and gz of a lump's pairs 2 h and 2 h + 1, and whether they are next to a ReLU's border (then zeros, if such are to be left out).
     template <bool LEFT_OUT>
-    __device__ __forceinline__ bool gz_told(const NormAct &p, float b_most, const float2 *mu, const float2 *a, const float2 *b, float2 *xc, float2 *out) {
-        float2 z[P];
-        Least least;
+    __device__ __forceinline__ bool gz_told(const NormAct &p, int h, float b_most, const float2 *mu, const float2 *a, const float2 *b, float2 *xc, float2 *out) {
+        constexpr int WORDS = Lump<T, VN>::WORDS / 2;
+        float2 z[2], rs[2];
 #pragma unroll
-        for (int j = 0; j < P; ++j) {
-            xc[j] = add2(pair_of(x.v[0], j), mu[j]);
-            z[j] = fma2(xc[j], a[j], b[j]);
-            if (p.residual) z[j] = add2(z[j], pair_of(res.v[0], j));
-            least.take(z[j]);
+        for (int i = 0; i < 2; ++i) {
+            const int j = 2 * h + i;
+            rs[i] = p.residual ? pair_of(res.v[0], j) : both(0.f);
+            xc[i] = add2(pair_of(x.v[0], j), mu[j]);
+            z[i] = fma2(xc[i], a[j], b[j]);
+            if (p.residual) z[i] = add2(z[i], rs[i]);
         }
-        const bool near = least.near(z, b, b_most, p.residual ? res.v[0].largest() : 0.f, [&](int j) { return p.residual ? pair_of(res.v[0], j) : both(0.f); });
+        const bool near = near_border(z, b + 2 * h, rs, b_most, p.residual ? res.v[0].largest_of_half(h) : 0.f);
         if (LEFT_OUT) {
 #pragma unroll
-            for (int w = 0; w < Lump<T, VN>::WORDS; ++w) g.v[0].w[w] = near ? 0u : g.v[0].w[w];
+            for (int w = 0; w < WORDS; ++w) g.v[0].w[WORDS * h + w] = near ? 0u : g.v[0].w[WORDS * h + w];
         }
 #pragma unroll
-        for (int j = 0; j < P; ++j) {
-            const float2 v = act2_backward<T>(ACT_RELU, z[j], pair_of(g.v[0], j));
-            out[j] = DROP ? drop2<VN>(p, words[0], j, v) : v;
+        for (int i = 0; i < 2; ++i) {
+            const float2 v = act2_backward<T>(ACT_RELU, z[i], pair_of(g.v[0], 2 * h + i));
+            out[i] = DROP ? drop2<VN>(p, words[0], 2 * h + i, v) : v;
         }
         return near;
     }
@@ -708,7 +707,7 @@ struct BackwardRows {
             float2 z = fma2(xc[j], a[j], b[j]);
             if (p.residual) z = add2(z, rs);
             if (SETTLED && act == ACT_RELU)
-                settle<VN>(p, s, c0 + 2 * (j0 + j), xs, b[j], rs, z);
+                settle_by_call<VN>(p, s, c0 + 2 * (j0 + j), xs, b[j], rs, z);
             const float2 v = act2_backward<T>(act, z, pair_of(g.v[u], j0 + j));
             out[j] = (DROP < 0 ? p.drop.on : DROP) ? drop2<VN>(p, words[u], j0 + j, v) : v;
         }
@@ -1028,7 +1027,7 @@ struct Piece { int kind, s, chunk, rows; };
 enum { ASK_NOTHING = 0, ASK_SUMS = 1, ASK_APPLY = 2, ASK_ANSWERED = 3 };
 // What passes between them, in the room of merge_groups (no block merges while one of its warps is at a tile).
 struct Asked {
-    uint32_t rounds[NA_THREADS];   // bit i: the i-th of the thread's rows in the tile
+    uint32_t rounds[NA_THREADS];   // bit 2 i + h: half h of the lump of the thread's i-th row in the tile (there are 12 at most)
     float2 sums[8][32];            // the answer: what those lumps add to a channel's sums
 };
 static_assert(sizeof(Asked) <= NA_THREADS * sizeof(double2), "room");
@@ -1213,8 +1212,8 @@ __device__ __forceinline__ void settle_tile(const NormAct &p, Ring &ring, const 
 #pragma unroll
     for (int j = 0; j < 4; ++j) a[j] = b[j] = both(0.f);
     uint32_t rounds = asked.rounds[32 * w + lane];
-    for (int at = l.lane * p.V; rounds; rounds >>= 1, at += l.lanes * p.V) {
-        if (!(rounds & 1)) continue;
+    for (int at = l.lane * p.V; rounds; rounds >>= 2, at += l.lanes * p.V) {
+        if (!(rounds & 3)) continue;
         const int64_t to = t.from + at + c0;
         const int first = PHASES ? t.first - at - c0 : 0, end = PHASES ? t.end - at - c0 : VN;
         BackwardRows<T, VN, ACT_RELU, DROP, 1> in;
@@ -1224,6 +1223,7 @@ __device__ __forceinline__ void settle_tile(const NormAct &p, Ring &ring, const 
         if (DROP) rng.template words<VN>((uint64_t)to, in.words[0]);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
+            if (kind == ASK_SUMS && !(rounds >> h & 1)) continue;
             float2 mu[2], fa[2], fb[2], m1[2], m2[2];
             k.read(l, K_MU, h, mu), k.read(l, K_A, h, fa), k.read(l, K_B, h, fb);
             if (kind == ASK_APPLY) k.read(l, K_M1, h, m1), k.read(l, K_M2, h, m2);
@@ -1267,7 +1267,8 @@ __device__ __forceinline__ void settle_tile(const NormAct &p, Ring &ring, const 
 template <typename T, int DROP, bool PHASES>
 __device__ __forceinline__ bool answer_until_folded(const NormAct &p, Ring &ring, const RingMemory &m, const Place &slot) {
     const int lane = threadIdx.x & 31;
-    for (uint64_t t0 = tc::global_timer_ns();;) {
+    uint64_t t0 = tc::global_timer_ns();
+    for (int turn = 0;; ++turn) {
         if (__all_sync(0xffffffffu, tc::mbar_try_wait_parked(tc::smem_u32(&ring.folded[slot.at]), slot.parity, 500u))) return true;
         const int asked = lane < NA_THREADS / 32 ? ring.asked[lane] & 3 : ASK_NOTHING;
         unsigned warps = __ballot_sync(0xffffffffu, asked == ASK_SUMS || asked == ASK_APPLY);
@@ -1275,6 +1276,7 @@ __device__ __forceinline__ bool answer_until_folded(const NormAct &p, Ring &ring
             for (; warps; warps &= warps - 1) settle_tile<T, DROP, PHASES>(p, ring, m, __ffs(warps) - 1);
             t0 = tc::global_timer_ns();
         }
+        if (turn % 64 != 63) continue;   // (each look at the clock is slow: at every turn, 179 us for 153 of 273 thousand rows of 256 channels, bf16)
         const bool late = tc::global_timer_ns() - t0 > tc::WAIT_LIMIT_NS, over = *const_cast<volatile int *>(&ring.abort);
         if (__any_sync(0xffffffffu, late || over)) {
             if (lane == 0 && !over) ring.abort = 1, atomicOr(p.status, NA_STATUS);
@@ -1345,7 +1347,7 @@ __device__ __forceinline__ void ring_clerk(const NormAct &p, Ring &ring, const R
 // meeting with that, whichever it is, and then all of them leave: a meeting is the first barrier that a warp comes to after any tile.
 template <typename T, int ACT, int DROP, bool BACKWARD, bool PHASES>
 __device__ __forceinline__ void ring_worker(const NormAct &p, Ring &ring, const RingMemory &m) {
-    constexpr int VN = 8, P = 4, UNROLL = DROP || (BACKWARD && ACT == ACT_RELU) ? 1 : 2;   // (more spills registers)
+    constexpr int VN = 8, P = 4;
     const Columns l(p.V, VN, threadIdx.x);
     const Folds<BACKWARD> folds(l);
     using Two = typename Folds<BACKWARD>::Two;
@@ -1483,23 +1485,27 @@ __device__ __forceinline__ void ring_worker(const NormAct &p, Ring &ring, const 
                 const T *x = rows_at();
                 uint32_t unsettled = 0, round = 1;
                 if (mine)
-#pragma unroll UNROLL
-                    for (int r = l.lane, at = l.lane * p.V; r < t.n; r += l.lanes, at += step, round <<= 1) {
+#pragma unroll 1   // (two at a time spill registers)
+                    for (int r = l.lane, at = l.lane * p.V; r < t.n; r += l.lanes, at += step, round <<= 2) {
                         BackwardRows<T, VN, ACT, DROP, 1> in;
                         in.x.v[0].load(x + at);
                         in.g.v[0].load(x + tensor + at);
                         if (p.residual) in.res.v[0].load(x + 2 * tensor + at);
                         if (DROP) rng.template words<VN>((uint64_t)(t.from + at + c0), in.words[0]);
-                        float2 xc[P], gz[P];
-                        if constexpr (ACT == ACT_RELU) unsettled |= in.template gz_told<true>(p, b_most, mu, fa, fb, xc, gz) ? round : 0;
-                        else in.template gz<P, false>(p, s, c0, 0, 0, mu, fa, fb, xc, gz);
-                        if (PHASES && cut(at + c0)) {
-                            const int2 e = ends();
+                        const bool part = PHASES && cut(at + c0);
 #pragma unroll
-                            for (int j = 0; j < P; ++j) xc[j] = within(xc[j], at + c0 + 2 * j, e.x, e.y), gz[j] = within(gz[j], at + c0 + 2 * j, e.x, e.y);
+                        for (int h = 0; h < 2; ++h) {
+                            float2 xc[2], gz[2];
+                            if constexpr (ACT == ACT_RELU) unsettled |= in.template gz_told<true>(p, h, b_most, mu, fa, fb, xc, gz) ? round << h : 0;
+                            else in.template gz<2, false>(p, s, c0, 0, 2 * h, mu + 2 * h, fa + 2 * h, fb + 2 * h, xc, gz);
+                            if (part) {
+                                const int2 e = ends();
+#pragma unroll
+                                for (int i = 0; i < 2; ++i) xc[i] = within(xc[i], at + c0 + 4 * h + 2 * i, e.x, e.y), gz[i] = within(gz[i], at + c0 + 4 * h + 2 * i, e.x, e.y);
+                            }
+#pragma unroll
+                            for (int i = 0; i < 2; ++i) a[2 * h + i] = add2(a[2 * h + i], gz[i]), b[2 * h + i] = fma2(gz[i], xc[i], b[2 * h + i]);
                         }
-#pragma unroll
-                        for (int j = 0; j < P; ++j) a[j] = add2(a[j], gz[j]), b[j] = fma2(gz[j], xc[j], b[j]);
                     }
                 bool lost = false;
                 if constexpr (ACT == ACT_RELU && BACKWARD)
@@ -1537,23 +1543,30 @@ __device__ __forceinline__ void ring_worker(const NormAct &p, Ring &ring, const 
                 if (!BACKWARD && t.last) k_apply.put_stats(p, l);
                 uint32_t unsettled = 0, round = 1;
                 if (mine)
-#pragma unroll UNROLL
-                    for (int r = l.lane, at = l.lane * p.V; r < t.n; r += l.lanes, at += step, round <<= 1) {
+#pragma unroll 1   // (two at a time spill registers)
+                    for (int r = l.lane, at = l.lane * p.V; r < t.n; r += l.lanes, at += step, round <<= 2) {
                         const int64_t to = t.from + at + c0;
                         BackwardRows<T, VN, ACT, DROP, 1> in;
                         in.x.v[0].load(x + at);
                         if constexpr (BACKWARD) in.g.v[0].load(x + tensor + at);
                         if (p.residual) in.res.v[0].load(x + (BACKWARD ? 2 : 1) * tensor + at);
                         if (DROP) rng.template words<VN>((uint64_t)to, in.words[0]);
-                        float2 xc[P], gz[P];
-                        if constexpr (BACKWARD && ACT == ACT_RELU) unsettled |= in.template gz_told<false>(p, b_most, mu, fa, fb, xc, gz) ? round : 0;
-                        else if constexpr (BACKWARD) in.template gz<P, false>(p, s, c0, 0, 0, mu, fa, fb, xc, gz);
+                        if constexpr (BACKWARD) {
 #pragma unroll
-                        for (int j = 0; j < P; ++j) {
-                            if constexpr (BACKWARD) {
-                                set_pair(in.g.v[0], j, gz[j]);
-                                set_pair(in.x.v[0], j, fma2(gz[j], fa[j], fma2(xc[j], m2[j], m1[j])));
-                            } else {
+                            for (int h = 0; h < 2; ++h) {
+                                float2 xc[2], gz[2];
+                                if constexpr (ACT == ACT_RELU) unsettled |= in.template gz_told<false>(p, h, b_most, mu, fa, fb, xc, gz) ? round << h : 0;
+                                else in.template gz<2, false>(p, s, c0, 0, 2 * h, mu + 2 * h, fa + 2 * h, fb + 2 * h, xc, gz);
+#pragma unroll
+                                for (int i = 0; i < 2; ++i) {
+                                    const int j = 2 * h + i;
+                                    set_pair(in.g.v[0], j, gz[i]);
+                                    set_pair(in.x.v[0], j, fma2(gz[i], fa[j], fma2(xc[i], m2[j], m1[j])));
+                                }
+                            }
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < P; ++j) {
                                 float2 z = fma2(add2(pair_of(in.x.v[0], j), mu[j]), fa[j], fb[j]);
                                 if (p.residual) z = add2(z, pair_of(in.res.v[0], j));
                                 z = act2<T>(ACT, z);

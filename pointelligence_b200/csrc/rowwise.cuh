@@ -118,16 +118,14 @@ struct Lump {
         for (int i = 0; i < VN; ++i)
             if (i >= first && i < end) p[i] = reinterpret_cast<const T *>(w)[i];
     }
-    // The largest magnitude of eight elements (NaN aside); of 16 bits by pairs.
-    __device__ __forceinline__ float largest() const {
+    // The largest magnitude of the elements 4 h .. 4 h + 3 of eight.
+    __device__ __forceinline__ float largest_of_half(int h) const {
         static_assert(VN == 8, "a whole lump");
-        if constexpr (sizeof(T) == 4) {
-            float m = 0.f;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(__uint_as_float(w[i])));
-            return m;
-        } else {   // (of values without a sign the order is that of whole numbers; a NaN is above them all)
-            const uint32_t m = __vmaxu2(__vmaxu2(w[0] & 0x7fff7fffu, w[1] & 0x7fff7fffu), __vmaxu2(w[2] & 0x7fff7fffu, w[3] & 0x7fff7fffu));
+        if constexpr (sizeof(T) == 4) {   // (NaN aside)
+            const float a = fmaxf(fabsf(__uint_as_float(w[4 * h])), fabsf(__uint_as_float(w[4 * h + 1]))), b = fmaxf(fabsf(__uint_as_float(w[4 * h + 2])), fabsf(__uint_as_float(w[4 * h + 3])));
+            return fmaxf(a, b);
+        } else {   // by pairs (of values without a sign the order is that of whole numbers; a NaN is above them all)
+            const uint32_t m = __vmaxu2(w[2 * h] & 0x7fff7fffu, w[2 * h + 1] & 0x7fff7fffu);
             const uint16_t v = (uint16_t)max(m & 0xffffu, m >> 16);
             return to_f32<T>(reinterpret_cast<const T &>(v));
         }
