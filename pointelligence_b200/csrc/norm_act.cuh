@@ -908,12 +908,12 @@ __device__ __forceinline__ void count_piece(const NormAct &p, const Span &v, int
     }
 }
 
-// dweight and dbias of some channels: the pieces' sums in a fixed order, in fp64 at last.
+// dweight and dbias of some channels: the pieces' sums in a fixed order, in fp64.  (There may be tens of thousands of them.)
 __device__ __noinline__ void affine_gradients(const NormAct &p, int tile, double2 *scratch) {
     constexpr int DEEP = NA_THREADS / AFFINE_CHANNELS;
     const int lane = threadIdx.x % AFFINE_CHANNELS, q = threadIdx.x / AFFINE_CHANNELS, c = tile * AFFINE_CHANNELS + lane;
     const int64_t pieces = p.N / p.rows + p.S;   // (numbers that no piece has hold zeros)
-    float a = 0.f, b = 0.f;
+    double a = 0.0, b = 0.0;
     if (c < p.C)
 #pragma unroll 8
         for (int64_t i = q; i < pieces; i += DEEP) {

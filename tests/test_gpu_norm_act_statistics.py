@@ -116,3 +116,21 @@ def test_no_sign_of_a_relu_is_on_the_other_side(points, samples, C, G, dtype, se
         gz = go.double() * (v * w.detach().double() + b.detach().double() + res.double() > 0)
         for got, want in ((db, gz.sum(0)), (dw, (gz * v).sum(0))):
             assert float((got.double() - want).norm() / want.norm()) <= 2.0 ** -20, seed
+
+
+def test_sums_of_pieces_are_of_64_bits():
+    """A large gradient in the first row and its opposite in the last: what lies between is summed beside them.  Sums of a piece are exact
+    here (multiples of 1/4 below 2^22, or one value and zeros), so that the bias's gradient is within its one rounding."""
+    from pointelligence_b200.layers.norm import fused_group_norm_act
+
+    N, C, edge = 3500003, 24, 200000
+    x = torch.randn(N, C, device=DEV).bfloat16()
+    go = torch.full_like(x, 0.25)
+    go[:edge] = 0
+    go[-edge:] = 0
+    go[0], go[-1] = 2.0 ** 30, -2.0 ** 30
+    w, b = torch.ones(C, device=DEV, requires_grad=True), torch.zeros(C, device=DEV, requires_grad=True)
+    y = fused_group_norm_act(x, torch.tensor([N], device=DEV), 4, w, b, activation="identity")
+    db, = torch.autograd.grad(y, b, go)
+    want = go.double().sum(0)
+    assert bool(((db.double() - want).abs() <= 2.0 ** -24 * want).all())
