@@ -94,9 +94,9 @@ int phase_bits_of(int C) {
 }
 
 // Rows of a chunk: 96 KB of them at most, and as many as give every block of the chip the same number of chunks, in whole rows of lanes.
-// (With two for a block wherever they were small, some blocks had two and some one: 20 thousand rows of 50 channels, fp32, 30 us
-// forward and 34 backward for 20 and 24, 5000 of 256, fp16, with dropout 28 and 32 for 22 and 28; with one, whatever 96 KB allow, 200
-// thousand of 96, bf16, 40 for 35.)
+// (With two for a block wherever they were small, some blocks had two and some one: 20 thousand rows of 50 channels, fp32, 34 us
+// forward and 36 backward for 24 and 26, 5000 of 256, fp16, with dropout 28 and 36 for 23 and 31; with one, whatever 96 KB allow, 200
+// thousand of 96, bf16, 45 for 40.)
 int chunk_rows(int64_t N, int C, int dtype) {
     const int bits = phase_bits_of(C);
     int vn = 8;
@@ -110,7 +110,7 @@ int chunk_rows(int64_t N, int C, int dtype) {
 // Pieces of a window: as many as leave a block NA_RECORDS records to read for itself, but not so many that the warp that merges a
 // window takes longer than all blocks with theirs: that time grows with the window, the blocks' with the number of windows, and at 1458
 // pieces they are alike at eight (one sample of 273 thousand rows, 256 instance norms, bf16, forward: windows of 4, 8, 16 and 46 (as
-// NA_RECORDS alone has it) pieces 187, 181, 203 and 278 us).
+// NA_RECORDS alone has it) pieces 178, 161, 178 and 247 us).
 int window_of(int chunks, int G) {
     const int64_t by_records = (chunks * (int64_t)G + NA_RECORDS - 1) / NA_RECORDS;
     const int64_t by_turns = std::max<int64_t>(8, (int64_t)std::sqrt(chunks / 24.0));
@@ -155,8 +155,8 @@ int run(const int64_t *d_lengths, NormAct &p, int dtype, int activation, std::in
     if (lump_of(p.V, dtype, tensors_at) == 8 && p.V <= RING_CHANNELS) {   // the ring
         const int lanes = Columns(p.V, 8, 0).lanes, tensors = (BACKWARD ? 2 : 1) + (p.residual ? 1 : 0), row_bytes = p.V * (int)elem_size(dtype);
         const int room = NA_RING_BYTES - (int)ring_bytes(p.V, p.G, BACKWARD);
-        // (Where two tiles of 24 KB do not fit, smaller ones: 1024 channels, bf16, backward 292 us of 70 million elements, 458 by the general
-        // kernel; where they do, three of two thirds are no better: 512 channels with a residual 230 and 252.)
+        // (Where two tiles of 24 KB do not fit, smaller ones: 1024 channels, bf16, backward 295 us of 70 million elements, 485 by the general
+        // kernel; where they do, three of two thirds are no better: 512 channels with a residual 248 and 250.)
         const int stage = room >= 2 * NA_STAGE_BYTES ? NA_STAGE_BYTES : room / 3;
         p.tile_rows = lanes * std::max(1, stage / (lanes * row_bytes * tensors));   // (at most 12 of a thread: lanes are more than half of the threads)
         p.sums_tile_rows = BACKWARD ? p.tile_rows : p.tile_rows * tensors;

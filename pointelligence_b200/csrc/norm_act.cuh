@@ -553,10 +553,11 @@ __device__ __forceinline__ float2 drop2(const NormAct &p, const uint32_t *words,
 }
 
 // ------------------------------------------------------------ signs ----
-// In the backward pass a ReLU's argument z = (t = (x - mu) a + b) + residual has its sign from fp64 where 32 bits do not settle it: on the other
-// side, an element would have a whole gradient too much or too little, and so would dbias and dweight.  (Forward it matters to no more than
-// a rounding, and costs 6 us of 115 for 1.1 million rows of 64 channels.)  With u = 2^-24, z is off by u (2 |(x - mu) a| + |b| + |t| + |z|) at most, which for a z near zero, where
-// |t| is next to |residual| and |(x - mu) a| below |t| + |b|, is 3 u (|b| + |residual|): z is settled beyond 4 u of these.
+// In the backward pass a ReLU's argument z = (t = (x - mu) a + b) + residual has its sign from fp64 where 32 bits do not settle it: on the
+// other side, an element would have a whole gradient too much or too little, and so would dbias and dweight.  (Forward it matters to no more
+// than a rounding: y is some 1e-8 there, or zero.  Settling it would cost 6 us of 115 for 1.1 million rows of 64 channels.)  With u = 2^-24,
+// z is off by u (2 |(x - mu) a| + |b| + |t| + |z|) at most, which for a z near zero, where |t| is next to |residual| and |(x - mu) a| at
+// most |t| + |b|, is 3 u (|b| + |residual|): z is settled beyond 4 u of these.
 constexpr float NEAR_BORDER = 0x1p-22f;
 __device__ __forceinline__ float exact_argument(const NormAct &p, int64_t s, int c, float x, float residual) {
     const int64_t g = s * p.G + group_of(p, c);
@@ -564,7 +565,8 @@ __device__ __forceinline__ float exact_argument(const NormAct &p, int64_t s, int
     return (float)((p.weight ? xh * __ldg(p.weight + c) + __ldg(p.bias + c) : xh) + residual);
 }
 __device__ __noinline__ float exact_argument_call(const NormAct &p, int64_t s, int c, float x, float residual) { return exact_argument(p, s, c, x, residual); }
-// Settles a pair of arguments where they are next to the border.
+// Settles a pair of arguments where they are next to the border.  (By a call where all elements come by, in the kernel without the ring: what
+// it would hold inline makes others spill, 1021 us for 979 of 34 thousand rows of 2048 channels, bf16, ReLU and residual, backward.)
 template <int VN>
 __device__ __forceinline__ void settle_by_call(const NormAct &p, int64_t s, int c, float2 x, float2 b, float2 residual, float2 &z) {
     if (fabsf(z.x) < NEAR_BORDER * (fabsf(b.x) + fabsf(residual.x))) z.x = exact_argument_call(p, s, channel_of(p, c), x.x, residual.x);
@@ -1003,11 +1005,13 @@ __global__ void __launch_bounds__(NA_THREADS, NA_BLOCKS) na_kernel(const __grid_
 // to be counted.
 //
 // Bound by bytes where the tail is short, every input read once a pass: 1.1 million points of 64 channels, bf16, eight samples, ReLU and
-// residual: forward 563 MB in 106 us, 5.3 TB/s; backward 1126 MB in 222 us, 5.1 TB/s, where 6.5 TB/s are a copy's.  By instructions with
-// SiLU and dropout of 0.1: 422 MB in 125 us, 704 MB in 225 us (without dropout 99 and 177).  Where all rows are some megabytes the
-// launch is latency: one sample of 942 points and 256 channels 12 to 15 us, of which a first read, the records' turn through the L2 and the
-// code's own way into the instruction cache are most.  (Lags of few chunks, so that the second pass finds its rows in the L2, do not pay:
-// what is in flight until a sample's records are there is as much as the L2 keeps beside what is written.)
+// residual: forward 563 MB in 113 us, 5.0 TB/s; backward 1126 MB in 224 us, 5.0 TB/s, where 6.5 TB/s are a copy's.  By instructions with
+// SiLU and dropout of 0.1: 422 MB in 134 us, 704 MB in 221 us (without dropout 105 and 166).  Forward, sums of 64 bits take the conversion
+// of each element, of which the chip does 16 a clock and SM: hidden behind 141 MB a tensor but for 5 us, and 2 of 40 us
+// where 38 MB are.  Where all rows are some megabytes the launch is latency: one sample of 942 points and 256 channels 12 to 15 us, of which
+// a first read, the records' turn through the L2 and the code's own way into the instruction cache are most.  (Lags of few chunks, so
+// that the second pass finds its rows in the L2, do not pay: what is in flight until a sample's records are there is as much as the L2
+// keeps beside what is written.)
 enum { TILE_SUMS = 0, TILE_APPLY = 1, TILE_AFFINE = 2, TILE_END = 3, TILE_NONE = 4 };
 constexpr int RING_CHANNELS = 1024;                // of a row, at most (their constants take room from the ring)
 constexpr int RING_STAGES = 8;                     // at most
@@ -1188,11 +1192,11 @@ __device__ __forceinline__ float2 within(float2 v, int at, int first, int end) {
     return make_float2(at >= first && at < end ? v.x : 0.f, at + 1 >= first && at + 1 < end ? v.y : 0.f);
 }
 
-// The clerk's answer to warp `w`: lane for lane what its threads would do, with the arguments' signs settled.  Lumps were left out of the sums; of
-// the results they are written once more.  Few elements come here (with a residual some ten of 70 million), but all may: values of 16
-// bits come again, and a channel's border may lie at one of them.  (The workers do not do it themselves: whatever they would hold
-// for it costs all other elements registers.  1.1 million points of 64 channels, bf16, residual, backward: 256 us where they do, 280 by a
-// call.)
+// The clerk's answer to warp `w`: lane for lane what its threads would do, with the arguments' signs settled.  Halves of lumps were left out
+// of the sums; of the results lumps are written once more.  Few elements come here (with a residual some ten of 70 million), but many may:
+// values of 16 bits come again, and a channel's border may lie at one of them (one channel of 64, 600 thousand rows a sample: 196 us for 170; all
+// channels, a seventh of their rows: 2.8 ms).  (The workers do not do it themselves: whatever they would hold for it costs all other
+// elements registers.  1.1 million points of 64 channels, bf16, residual, backward: 222 us, 256 where they do, 280 by a call.)
 template <typename T, int DROP, bool PHASES>
 __device__ __forceinline__ void settle_tile(const NormAct &p, Ring &ring, const RingMemory &m, int w) {
     constexpr int VN = 8;
@@ -1607,7 +1611,7 @@ __device__ __forceinline__ void ring_worker(const NormAct &p, Ring &ring, const 
 }
 
 // PHASES: several rows side by side.  (Always so, the samples' ends cost registers where none is inside of a row: at 1.1 million points of
-// 64 channels, bf16, 252 us backward for 222 and 114 forward for 106.)
+// 64 channels, bf16, 236 us backward for 221 and 118 forward for 107.)
 template <typename T, int ACT, int DROP, bool BACKWARD, bool PHASES>
 __global__ void __launch_bounds__(RING_THREADS, RING_BLOCKS) na_ring_kernel(const __grid_constant__ NormAct p) {
     extern __shared__ __align__(128) char shared[];
