@@ -83,6 +83,21 @@ def _at_the_border(lengths, C, G, dtype, residual, seed):
 def test_signs_at_the_border(C, G, lengths, dtype, residual, p):
     """Every element of the gradients of x and of the residual, and of the sums, is on the side that float64 gives it; y is the ReLU of an
     argument that is off by some 2^-22 of its terms."""
+    _check_signs(C, G, lengths, dtype, residual, p, (5, 8) if p else None)
+
+
+@pytest.mark.parametrize("C,G", [(8, 2), (24, 3), (100, 4), (130, 13), (512, 8), (688, 1), (1000, 5), (1024, 32)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_signs_at_the_border_of_other_widths(C, G, dtype):
+    """With a seed on the device; no wait of a kernel runs out."""
+    from pointelligence_b200 import _cabi
+
+    _check_signs(C, G, [1700, 2, 640], dtype, True, 0.3, torch.tensor([5, 8], device=DEV))
+    _check_signs(C, G, [1700, 2, 640], dtype, False, 0.0, None)
+    assert _cabi.device_status() == 0
+
+
+def _check_signs(C, G, lengths, dtype, residual, p, rng):
     import numpy as np
 
     from oracle import norm_act as oracle
@@ -92,7 +107,7 @@ def test_signs_at_the_border(C, G, lengths, dtype, residual, p):
     N = sum(lengths)
     go = (1 + torch.rand(N, C, device=DEV)).to(dtype)      # (no gradient is zero)
     leaves = [t.requires_grad_() for t in (x, w, b)] + ([res.requires_grad_()] if residual else [])
-    y = fused_group_norm_act(x, torch.tensor(lengths, device=DEV), G, w, b, residual=res, activation="relu", dropout=p, rng=(5, 8) if p else None)
+    y = fused_group_norm_act(x, torch.tensor(lengths, device=DEV), G, w, b, residual=res, activation="relu", dropout=p, rng=rng)
     grads = torch.autograd.grad(y, leaves, go)
     _, rstd, xh, z = _definition(x.detach(), lengths, G, w.detach(), b.detach(), None if res is None else res.detach())
     near = z.abs() < 2.0 ** -22
@@ -202,3 +217,35 @@ def test_not_a_number_stays_in_its_channel(kind, C):
         apart[3::8] = apart[6::8] = False
         for a, b in zip(run(bad_x, bad_res), clean):
             assert torch.equal(a[:, apart], b[:, apart])
+
+
+def test_signs_on_two_streams_and_in_a_replayed_graph():
+    """The same bits as alone, with many elements at the border."""
+    from pointelligence_b200 import _cabi
+    from pointelligence_b200.layers.norm import fused_group_norm_act
+
+    cases = []
+    for C, G, lengths in ((64, 8, [20000, 9000]), (50, 5, [15000, 3, 12000])):
+        x, res, w, b = _at_the_border(lengths, C, G, torch.bfloat16, True, C)
+        leaves = [t.requires_grad_() for t in (x, w, b, res)]
+        go, lens = torch.randn_like(x), torch.tensor(lengths, device=DEV)
+        cases.append(lambda leaves=leaves, go=go, lens=lens, G=G: torch.autograd.grad(
+            fused_group_norm_act(leaves[0], lens, G, leaves[1], leaves[2], residual=leaves[3], activation="relu", dropout=0.1, rng=(1, 4)), leaves, go))
+    alone = [step() for step in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    for _ in range(4):
+        got = []
+        for stream, step in zip(streams, cases):
+            with torch.cuda.stream(stream):
+                got.append(step())
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for q, r in zip(alone, got) for a, b in zip(q, r))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = [step() for step in cases]
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for q, r in zip(alone, out) for a, b in zip(q, r))
+    assert _cabi.device_status() == 0
